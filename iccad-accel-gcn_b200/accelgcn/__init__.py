@@ -9,6 +9,8 @@ of libaccelgcn.so (include/accelgcn.h).
     sharded     -- 1D row-sharded multi-GPU SpMM (agcn_dist_*: layout, NCCL exchange and kernels in the library)
     gcn         -- two-layer GCN forward on the row blocks (agcn_gcn2_forward_*)
     gemm        -- dense feature transform on the tensor cores (agcn_gemm_tf32*)
+    norm        -- layer norm with ReLU and dropout behind it, and its gradients (agcn_layer_norm*)
+    dropout     -- dropout with a mask made from a counter, and its gradient (agcn_dropout*)
 
 PyTorch appears here only as the owner of device memory and streams (and of the
 process group in `sharded`); all compute is in the shared library.

@@ -20,7 +20,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_CAPACITY, ERR_RANGE = 0, -1, -2, -3, -4
 DEG_BOUND = 384
 PARTITION_NOALLOC_MAX_ROWS = 1 << 24
 
-_vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_vp, _i64, _int, _f64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double
 
 # name -> (restype, argtypes); every symbol include/accelgcn.h declares
 PROTOTYPES = {
@@ -82,6 +82,12 @@ PROTOTYPES = {
     "agcn_gcn2_forward_launches": (_int, [_vp, ctypes.POINTER(_int)]),
     "agcn_gcn2_forward_paired": (_int, [_vp, ctypes.POINTER(_int)]),
     "agcn_gcn2_forward_destroy": (_int, [_vp]),
+    "agcn_layer_norm": (_int, [_vp, _i64, _vp, _vp, _f64, _vp, _i64, _vp, _i64, _i64, _int, _int, _f64, _i64, _i64, _vp, _i64, _vp]),
+    "agcn_layer_norm_backward_work": (_int, [_i64, _i64, _int, ctypes.POINTER(_i64)]),
+    "agcn_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _f64, _i64,
+                                        _i64, _vp, _i64, _vp]),
+    "agcn_dropout": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _int, _f64, _i64, _i64, _vp, _i64, _vp]),
+    "agcn_dropout_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _int, _int, _f64, _i64, _i64, _vp, _i64, _vp]),
     "agcn_probe_gather_bandwidth": (_int, [_i64, _int, _i64, _int, _int, ctypes.POINTER(ctypes.c_double)]),
 }
 DIST_ID_BYTES = 128
@@ -121,7 +127,7 @@ def load():
 
 
 def call():
-    """The native caller `call(address, *integers) -> int` (csrc/pycall.c): what the hot paths use in place of
+    """The native caller `call(address, *integers_and_doubles) -> int` (csrc/pycall.c): what the hot paths use in place of
     ctypes.  No fallback: it is built with the library."""
     global _call
     if _call is None:

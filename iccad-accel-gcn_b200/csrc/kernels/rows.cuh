@@ -1,0 +1,137 @@
+// Rows of features in 32 or 16 bits, 16 bytes per thread at a time: what the layer norm and dropout kernels share.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace agcn {
+
+// E elements of type T are 16 bytes.  All arithmetic is in fp32; the one rounding to T is that of the result.
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ float get(float v) { return v; }
+    static __device__ __forceinline__ float put(float v) { return v; }
+    static __device__ __forceinline__ void unpack(const uint4 &r, float *v)
+    {
+        v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float *v)
+    {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4 &r, float *v)
+    {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) { v[2 * k] = __uint_as_float(w[k] << 16); v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ uint4 pack(const float *v)
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Elem<__half> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4 &r, float *v)
+    {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+            v[2 * k] = f.x; v[2 * k + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float *v)
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// Columns c0 .. c0 + E - 1 of a row, as far as they are in [0, cols); zeros elsewhere.  VEC: a whole chunk is one access
+// (column c0 then sits on a 16-byte boundary); the chunks at the ends of a row go element by element, so that nothing
+// outside the row is touched.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T *row, int c0, int cols, float *v)
+{
+    constexpr int E = Elem<T>::E;
+    if (VEC && c0 >= 0 && c0 + E <= cols) {
+        Elem<T>::unpack(*reinterpret_cast<const uint4 *>(row + c0), v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = c0 + e >= 0 && c0 + e < cols ? Elem<T>::get(row[c0 + e]) : 0.f;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_chunk(T *row, int c0, int cols, const float *v)
+{
+    constexpr int E = Elem<T>::E;
+    if (VEC && c0 >= 0 && c0 + E <= cols) {
+        *reinterpret_cast<uint4 *>(row + c0) = Elem<T>::pack(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) if (c0 + e >= 0 && c0 + e < cols) row[c0 + e] = Elem<T>::put(v[e]);
+    }
+}
+
+// max(v, 0) that lets NaN through, and whether a gradient passes
+__device__ __forceinline__ float relu_of(float v) { return v < 0.f ? 0.f : v; }
+__device__ __forceinline__ bool relu_passes(float v) { return !(v <= 0.f); }
+
+// Sums of K values over a group of L lanes of a warp, or (L = 0) over the thread block; every thread gets them, added
+// in one order.  All lanes of the warp (threads of the block) call.  s_sums: zero where there is no warp; `turn` says which half is
+// free: the other one may still be read by warps that are behind.
+constexpr int ROW_WARPS = 20;              // most warps of a thread block that has one row, a multiple of 4
+template <int K> struct GroupSums { alignas(16) float v[2][K][ROW_WARPS]; };
+template <int K>
+__device__ __forceinline__ void clear_sums(GroupSums<K> &s)
+{
+    for (int i = threadIdx.x; i < 2 * K * ROW_WARPS; i += blockDim.x) (&s.v[0][0][0])[i] = 0.f;
+}
+template <int L, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], GroupSums<K> &s_sums, int &turn)
+{
+    constexpr int W = L > 0 ? L : 32;
+#pragma unroll
+    for (int d = W / 2; d > 0; d >>= 1) {
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], d);
+    }
+    if (L == 0) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; k++) s_sums.v[turn][k][threadIdx.x >> 5] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const float4 *q = reinterpret_cast<const float4 *>(s_sums.v[turn][k]);
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < ROW_WARPS / 4; i++) s += (q[i].x + q[i].y) + (q[i].z + q[i].w);
+            v[k] = s;
+        }
+        turn ^= 1;
+    }
+}
+
+}  // namespace agcn

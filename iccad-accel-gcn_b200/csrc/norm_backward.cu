@@ -1,0 +1,98 @@
+// Gradients of layer norm, ReLU and dropout (norm.cu) in one pass over the rows, and the column sums.
+#include "norm.h"
+
+namespace agcn {
+
+// Thread blocks per SM whose sums the workspace holds: all that are resident, for the forms there are
+static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int sms)
+{
+    const int64_t chunks = ceil_div(cols, 16 / dtype_bytes(dtype)), per_warp = 32 * NORM_ELEMS / (16 / dtype_bytes(dtype));
+    const int64_t threads = chunks <= per_warp ? NORM_THREADS : 32 * ceil_div(chunks, per_warp);
+    const int64_t most = sms * (2048 / threads);
+    return rows < most ? (rows > 0 ? rows : 1) : most;
+}
+
+struct NormBackwardLaunch {
+    NormBackward &p;
+    const NormForm &f;
+    float *work;
+    int64_t most_parts;
+    cudaStream_t s;
+    template <typename T, int L, int CH, bool VEC> int operator()() const
+    {
+        int64_t resident = 0;
+        const int rc = norm_resident<layer_norm_backward_kernel<T, L, CH, VEC>>(f.threads, &resident);
+        if (rc != AGCN_OK) return rc;
+        float *dweight = p.dweight, *dbias = p.dbias;
+        const int64_t grid = norm_grid(f, p.rows, resident < most_parts ? resident : most_parts);
+        const bool sums = (dweight != nullptr || dbias != nullptr) && grid > 1;
+        AGCN_REQUIRE(!sums || grid <= most_parts, "agcn_layer_norm_backward: the workspace is too small");
+        if (sums) {
+            p.part_stride = 2 * p.cols;
+            p.dweight = dweight != nullptr ? work : nullptr;
+            p.dbias = dbias != nullptr ? work + p.cols : nullptr;
+        }
+        layer_norm_backward_kernel<T, L, CH, VEC><<<(unsigned)grid, f.threads, 0, s>>>(p);
+        AGCN_LAUNCH_CHECK("layer_norm_backward_kernel");
+        if (sums) {
+            norm_columns_kernel<<<dim3((unsigned)ceil_div(p.cols, 32), 2), 256, 0, s>>>(work, p.part_stride, (int)grid, dweight, dbias, p.cols);
+            AGCN_LAUNCH_CHECK("norm_columns_kernel");
+        }
+        return AGCN_OK;
+    }
+};
+
+}  // namespace agcn
+
+extern "C" int agcn_layer_norm_backward_work(int64_t rows, int64_t cols, int dtype, int64_t *bytes)
+{
+    using namespace agcn;
+    clear_error();
+    const char *who = "agcn_layer_norm_backward_work";
+    AGCN_REQUIRE(bytes != nullptr, "%s: null result pointer", who);
+    int dev = 0, sms = 0;
+    int rc = check_sizes(who, rows, cols, NORM_MAX_COLS, dtype, AGCN_ACT_NONE);
+    if (rc == AGCN_OK) rc = current_sm_count(&dev, &sms);
+    if (rc == AGCN_OK) *bytes = norm_parts(rows, cols, dtype, sms) * 2 * cols * (int64_t)sizeof(float);
+    return rc;
+}
+
+extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const float *d_stats, const float *d_weight,
+                                        const float *d_bias, void *d_dx, int64_t lddx, float *d_dweight, float *d_dbias, void *d_work,
+                                        int64_t work_bytes, int64_t rows, int64_t cols, int dtype, int activation, double p, int64_t seed,
+                                        int64_t offset, const int64_t *d_step, int64_t row0, void *stream)
+{
+    using namespace agcn;
+    clear_error();
+    const char *who = "agcn_layer_norm_backward";
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    NormBackward a = {};
+    int rc = check_sizes(who, rows, cols, NORM_MAX_COLS, dtype, activation);
+    if (rc == AGCN_OK) rc = make_mask(who, &a.mask, p, seed, offset, d_step, row0, rows, cols);
+    if (rc != AGCN_OK) return rc;
+    AGCN_REQUIRE(aligned4(d_weight) && aligned4(d_bias) && aligned4(d_dweight) && aligned4(d_dbias) && aligned4(d_work) &&
+                     reinterpret_cast<uintptr_t>(d_stats) % 8 == 0,
+                 "%s: weight, bias, their gradients and the workspace must be aligned to 4 bytes, stats to 8", who);
+    if (rows == 0) {
+        if (d_dweight != nullptr) AGCN_CUDA(cudaMemsetAsync(d_dweight, 0, (size_t)cols * sizeof(float), s));
+        if (d_dbias != nullptr) AGCN_CUDA(cudaMemsetAsync(d_dbias, 0, (size_t)cols * sizeof(float), s));
+        return AGCN_OK;
+    }
+    AGCN_REQUIRE(d_stats != nullptr, "%s: stats is null", who);
+    const Rows t[3] = {{d_dy, lddy, "dy"}, {d_x, ldx, "x"}, {d_dx, lddx, "dx"}};
+    for (const Rows &r : t)
+        if ((rc = check_rows(who, r, rows, cols, dtype)) != AGCN_OK) return rc;
+    int dev = 0, sms = 0;
+    if ((rc = current_sm_count(&dev, &sms)) != AGCN_OK) return rc;
+    const int64_t parts = norm_parts(rows, cols, dtype, sms);
+    AGCN_REQUIRE((d_dweight == nullptr && d_dbias == nullptr) || (d_work != nullptr && work_bytes >= parts * 2 * cols * (int64_t)sizeof(float)),
+                 "%s: workspace of %lld bytes, %lld are needed", who, (long long)work_bytes, (long long)(parts * 2 * cols * (int64_t)sizeof(float)));
+    a.dy = d_dy; a.lddy = lddy; a.x = d_x; a.ldx = ldx; a.dx = d_dx; a.lddx = lddx; a.rows = rows;
+    a.weight = d_weight; a.bias = d_bias;
+    a.stats = reinterpret_cast<const float2 *>(d_stats);
+    a.dweight = d_dweight; a.dbias = d_dbias;
+    a.cols = (int)cols; a.relu = activation == AGCN_ACT_RELU;
+    a.inv_cols = 1.f / (float)cols;
+    const NormForm f = norm_form(t, 3, cols, dtype, a.mask.on);
+    return norm_dispatch(f, dtype, NormBackwardLaunch{a, f, static_cast<float *>(d_work), parts, s});
+}

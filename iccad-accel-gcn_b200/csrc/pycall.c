@@ -3,23 +3,29 @@
  *
  *   call(address, a, b, ...) -> int
  *
- * calls the function at `address` with up to 14 integer or pointer arguments (None is a null pointer) and returns
- * its int.  Every parameter of the C ABI is an integer or a pointer, and on this ABI (x86-64 and AArch64 System V)
- * those all travel as 64-bit values in the same places. */
+ * calls the function at `address` with up to 24 integer or pointer arguments (None is a null pointer) and up to 4
+ * doubles (Python floats), and returns its int.  Every parameter of the C ABI is an integer, a pointer or a double; on
+ * this ABI (x86-64 and AArch64 System V) integers and pointers all travel as 64-bit values in the same places, and
+ * doubles in registers of their own, wherever they stand among the others. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#define MAX_ARGS 14
-typedef int (*fn_t)(long, long, long, long, long, long, long, long, long, long, long, long, long, long);
+#define MAX_ARGS 24
+#define MAX_DOUBLES 4
+#define TEN_LONGS long, long, long, long, long, long, long, long, long, long
+typedef int (*few_t)(TEN_LONGS, long, long, long, long);
+typedef int (*many_t)(double, double, double, double, TEN_LONGS, TEN_LONGS, long, long, long, long);
 
 static PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n)
 {
     long a[MAX_ARGS] = {0};
+    double d[MAX_DOUBLES] = {0};
+    int longs = 0, doubles = 0;
     void *address;
     int rc;
     (void)self;
-    if (n < 1 || n > MAX_ARGS + 1) {
-        PyErr_SetString(PyExc_TypeError, "call(address, up to 14 integers)");
+    if (n < 1 || n > MAX_ARGS + MAX_DOUBLES + 1) {
+        PyErr_SetString(PyExc_TypeError, "call(address, up to 24 integers and 4 doubles)");
         return NULL;
     }
     address = PyLong_AsVoidPtr(args[0]);
@@ -28,18 +34,31 @@ static PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n)
         return NULL;
     }
     for (Py_ssize_t i = 1; i < n; i++) {
-        if (args[i] == Py_None) continue;
-        a[i - 1] = PyLong_AsLong(args[i]);
-        if (a[i - 1] == -1 && PyErr_Occurred()) return NULL;
+        if (PyFloat_CheckExact(args[i]) ? doubles == MAX_DOUBLES : longs == MAX_ARGS) {
+            PyErr_SetString(PyExc_TypeError, "call(address, up to 24 integers and 4 doubles)");
+            return NULL;
+        }
+        if (PyFloat_CheckExact(args[i])) {
+            d[doubles++] = PyFloat_AS_DOUBLE(args[i]);
+            continue;
+        }
+        if (args[i] == Py_None) { longs++; continue; }
+        a[longs] = PyLong_AsLong(args[i]);
+        if (a[longs] == -1 && PyErr_Occurred()) return NULL;
+        longs++;
     }
     Py_BEGIN_ALLOW_THREADS
-    rc = ((fn_t)address)(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13]);
+    if (longs <= 14 && doubles == 0)
+        rc = ((few_t)address)(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13]);
+    else
+        rc = ((many_t)address)(d[0], d[1], d[2], d[3], a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11],
+                               a[12], a[13], a[14], a[15], a[16], a[17], a[18], a[19], a[20], a[21], a[22], a[23]);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
 }
 
 static PyMethodDef methods[] = {
-    {"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, *integers) -> int"},
+    {"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, *integers_and_doubles) -> int"},
     {NULL, NULL, 0, NULL},
 };
 

@@ -442,6 +442,62 @@ int agcn_gcn2_forward_paired(const agcn_gcn2 *fwd, int *paired);
 int agcn_gcn2_forward_destroy(agcn_gcn2 *fwd);
 
 /* ------------------------------------------------------------------------
+ * The row-wise part of a GCN layer that is trained (or served as it was trained): layer norm, ReLU and dropout
+ * between one product A * Z and the next transform, with their gradients.  No counterpart in the reference, which
+ * stops at the SpMM (spmm_accel.cu:104-108).
+ *
+ * Features are [rows x cols] of type `dtype`, row-major, row strides ld >= cols in ELEMENTS, any alignment that the
+ * elements have (rows of all tensors that sit alike with respect to 16-byte boundaries are read 16 bytes at a time,
+ * others element by element; between layouts, sums may be made in another order).  Statistics, sums, weights and their gradients are fp32, and
+ * so is all arithmetic; a result is rounded to `dtype` once.  An output may be an input of the same call with the
+ * same stride (y = x, dx = dy or x); other overlaps are not allowed.  All calls are asynchronous on `stream`,
+ * allocate nothing and may be captured.  rows = 0 is allowed.
+ * AGCN_ACT_RELU: max(., 0); NaN stays NaN here (so a broken step shows), its gradient passes.
+ *
+ * Dropout: 0 <= p < 1.  Element (r, c) has the number i = (row0 + r) * cols + c and is kept if word i % 4 of
+ * Philox4x32-10 with the 128-bit counter (i / 4, offset + *d_step), low half first, and the key `seed` is at least
+ * floor(p * 2^32); what is kept is multiplied by 1 / (1 - p), the rest is 0 whatever it was (NaN and infinities
+ * included).  The mask is never stored: the backward pass gets the same numbers and makes it again.  Give every layer
+ * and every step another `offset` (or seed).  d_step (optional, one device int64) is read when the kernel runs: what a
+ * captured graph counts up to have another mask at each replay.  row0: where this rank's rows begin, so that the mask of
+ * a row-sharded step is that of the whole.  p = 0: everything is kept and nothing is drawn.
+ * ---------------------------------------------------------------------- */
+#define AGCN_F32  0
+#define AGCN_BF16 1
+#define AGCN_F16  2
+#define AGCN_NORM_MAX_COLS 8192
+
+/* y = dropout(act((x - m) s * weight + bias)),  m and s = 1 / sqrt(variance + eps) those of each row of x (the variance
+ * divides by cols).  weight / bias [cols] fp32, NULL: 1 / 0.  d_stats: NULL, or fp32 [rows x 2], contiguous, which
+ * receives (m, s) for the backward pass.  1 <= cols <= AGCN_NORM_MAX_COLS.  Squares are taken in fp32: deviations from
+ * the mean of 1e19 and more overflow. */
+int agcn_layer_norm(const void *d_x, int64_t ldx, const float *d_weight, const float *d_bias, double eps,
+                    void *d_y, int64_t ldy, float *d_stats, int64_t rows, int64_t cols, int dtype, int activation,
+                    double p, int64_t seed, int64_t offset, const int64_t *d_step, int64_t row0, void *stream);
+
+/* Its gradients, from dy, the x, stats, weight and bias of the forward pass, and the same activation and mask:
+ * d_dx [rows x cols] of `dtype`, d_dweight and d_dbias [cols] fp32 (overwritten; either may be NULL).  The sums over
+ * the rows are made in one order: the same bits from run to run on one GPU model.  d_work: fp32 workspace of at least
+ * agcn_layer_norm_backward_work(...) bytes (what the current device needs), whose contents mean nothing before and
+ * after; calls that may overlap need one each.  NULL where neither d_dweight nor d_dbias is wanted. */
+int agcn_layer_norm_backward_work(int64_t rows, int64_t cols, int dtype, int64_t *bytes);
+int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const float *d_stats,
+                             const float *d_weight, const float *d_bias, void *d_dx, int64_t lddx,
+                             float *d_dweight, float *d_dbias, void *d_work, int64_t work_bytes,
+                             int64_t rows, int64_t cols, int dtype, int activation,
+                             double p, int64_t seed, int64_t offset, const int64_t *d_step, int64_t row0, void *stream);
+
+/* y = dropout(act(x)), any number of columns; for a product whose ReLU is fused already: AGCN_ACT_NONE. */
+int agcn_dropout(const void *d_x, int64_t ldx, void *d_y, int64_t ldy, int64_t rows, int64_t cols, int dtype,
+                 int activation, double p, int64_t seed, int64_t offset, const int64_t *d_step, int64_t row0, void *stream);
+
+/* Its gradient: dx = dy / (1 - p) where the element was kept (and x > 0, with AGCN_ACT_RELU: d_x is then the forward
+ * pass's x, or relu(x); otherwise it is not used and may be NULL), else 0. */
+int agcn_dropout_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, void *d_dx, int64_t lddx,
+                          int64_t rows, int64_t cols, int dtype, int activation,
+                          double p, int64_t seed, int64_t offset, const int64_t *d_step, int64_t row0, void *stream);
+
+/* ------------------------------------------------------------------------
  * Measurement aid (not on the product path): the rate, in GB/s, at which this
  * GPU gathers whole rows of an L2-resident table with the access shape of the
  * SpMM (16-byte lanes, four rows in flight per lane, same residency and L2
