@@ -39,15 +39,16 @@ dropout_kernel(const __grid_constant__ DropoutParams p)
             float v[E], gate[E];
             load_chunk<T, VEC>(v_row + at, lo, left, v);
             if (p.gate != nullptr) load_chunk<T, VEC>(gate_row + at, lo, left, gate);
-            const uint32_t keep = p.mask.on ? keep_bits<E>(p.mask, offset, first + c0) : ~0u;
+            uint32_t word[1][E];
+            if (p.mask.on) draw_words<1, E>(p.mask, offset, (first + c0) >> 2, 0, (int)((first + c0) & 3), word);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 float x = v[e];
                 if (p.relu) x = relu_of(x);
                 if (p.mask.on) x *= p.mask.scale;
-                v[e] = (keep >> e & 1u) && (p.gate == nullptr || relu_passes(gate[e])) ? x : 0.f;
+                v[e] = (!p.mask.on || word[0][e] >= p.mask.threshold) && (p.gate == nullptr || relu_passes(gate[e])) ? x : 0.f;
             }
-            store_chunk<T, VEC>(out_row + at, lo, left, v);
+            store_chunk<T, VEC, false>(out_row + at + lo, lo, left, v);
         }
     }
 }

@@ -9,18 +9,29 @@
 // registers, CH chunks of 16 bytes per lane, so every element is read once; rows go round-robin over the groups.  The
 // number of groups is a multiple of 8, so a group's rows all sit at one offset from a 16-byte boundary and a lane has the
 // same columns in all of them: weights and the sums over the rows stay in registers, and rows of any width are read 16
-// bytes at a time (VEC; rows of tensors that do not sit alike are read element by element).
+// bytes at a time (rows of tensors that do not sit alike are read element by element).  The next rows are under way
+// in a ring in shared memory meanwhile (RowRing).
 #pragma once
 #include "philox.cuh"
 #include "rows.cuh"
 
 namespace agcn {
 
+constexpr int NORM_STAGES = 3;             // rows ahead in the ring
 constexpr int NORM_THREADS = 256;          // of the forms with several rows per thread block
 constexpr int NORM_MAX_THREADS = 544;      // of the form with one: 8192 columns, 16 per thread, from any offset on
 static_assert(NORM_MAX_THREADS <= 32 * ROW_WARPS, "group_sum holds the sums of that many warps");
 
+// The rows of a call over the groups: every group has `turns` of them, the first `rest` groups one more.
+struct NormRows {
+    int turns;
+    int64_t rest;
+    int64_t words;                         // of the mask, in blocks, from one row of a group to its next
+};
+
 struct NormForward {
+    NormRows part;
+    int64_t x_step, y_step;                // elements from one row of a group to its next
     const void *x;
     void *y;
     int64_t ldx, ldy, rows;
@@ -32,6 +43,8 @@ struct NormForward {
 };
 
 struct NormBackward {
+    NormRows part;
+    int64_t dy_step, x_step, dx_step;
     const void *dy, *x;
     void *dx;
     int64_t lddy, ldx, lddx, rows;
@@ -44,21 +57,80 @@ struct NormBackward {
     DropoutMask mask;
 };
 
-// Elements that the first of a group's columns stands behind a 16-byte boundary (VEC), or behind a whole block of the
-// mask's words; the same for all rows of the group.
-template <typename T, bool VEC>
-__device__ __forceinline__ int row_shift(const void *x, int64_t ldx, const DropoutMask &mask, int cols, int64_t row)
+// How the rows of all tensors of a call sit: alike with respect to 16-byte boundaries, every row beginning and ending on
+// one (WHOLE); alike, with chunks at the rows' ends that are not the row's alone (EDGES); or not alike (LOOSE: read
+// element by element).
+enum RowLayout { ROWS_WHOLE, ROWS_EDGES, ROWS_LOOSE };
+
+// Where a thread of a layer norm kernel stands.
+template <typename T, int L, int CH, int LAYOUT>
+struct NormPlace {
+    static constexpr int E = Elem<T>::E;
+    int lanes, t;                        // threads of the group, this one's number
+    int64_t group, groups;
+    int turns, warp_turns;               // rows of the group; the most that a group of this warp has
+    int shift;                           // elements that the group's rows begin behind a boundary: of 16 bytes, or (LOOSE) of the mask's blocks
+    uint32_t ok;                         // which of the thread's CH * E columns there are
+    __device__ __forceinline__ NormPlace(const NormRows &part, const void *x, int64_t ldx, int cols, const DropoutMask &mask)
+    {
+        lanes = L > 0 ? L : (int)blockDim.x;
+        t = L > 0 ? (int)threadIdx.x & (L - 1) : (int)threadIdx.x;
+        groups = (int64_t)gridDim.x * (L > 0 ? NORM_THREADS / (L > 0 ? L : 1) : 1);
+        group = L > 0 ? ((int64_t)blockIdx.x * NORM_THREADS + threadIdx.x) / (L > 0 ? L : 1) : (int64_t)blockIdx.x;
+        turns = part.turns + (group < part.rest);
+        warp_turns = L > 0 ? part.turns + (group - ((int)threadIdx.x & 31) / (L > 0 ? L : 1) < part.rest) : turns;
+        shift = 0;
+        if (LAYOUT == ROWS_EDGES) shift = (int)(((int64_t)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) + group * ldx) & (E - 1));
+        if (LAYOUT == ROWS_LOOSE && mask.on) shift = (int)((mask.first + group * cols) & 3);
+        ok = 0;
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (column(j) + e >= 0 && column(j) + e < cols) ok |= 1u << (j * E + e);
+    }
+    __device__ __forceinline__ int column(int j) const { return (j * lanes + t) * E - shift; }
+    // All ones where the thread has the column (WHOLE: a chunk is there or not; a slot of the ring that is never filled is 0)
+    __device__ __forceinline__ uint32_t mine(int j, int e) const { return 0u - (ok >> (j * E + (LAYOUT == ROWS_WHOLE ? 0 : e)) & 1u); }
+    __device__ __forceinline__ bool has(int j) const { return ok >> (j * E) & ((1u << E) - 1); }
+    // Starts the copies of a row's chunks, from where this thread's first one is.
+    template <int N, int STAGES>
+    __device__ __forceinline__ void fetch(const RowRing<T, N, CH, STAGES> &ring, int k, const T *from, const T *first, int cols) const
+    {
+#pragma unroll
+        for (int j = 0; j < CH; j++) {
+            if (!has(j)) continue;
+            if (LAYOUT == ROWS_WHOLE) ring.fetch(k, j, from + j * lanes * E);
+            else {
+                const int n = cols - column(j);
+                ring.fetch_edge(k, j, from + j * lanes * E, first, column(j), cols, n >= E ? 16 : n * (int)sizeof(T));
+            }
+        }
+    }
+    // Stores a row's chunks, to where this thread's first one is.
+    template <bool VEC>
+    __device__ __forceinline__ void store(T *to, int cols, const float (&v)[CH][E]) const
+    {
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+            if (has(j)) store_chunk<T, VEC, LAYOUT == ROWS_WHOLE>(to + j * lanes * E, column(j), cols, v[j]);
+    }
+};
+
+// 1 / sqrt(v): the approximation and one step of Newton's method, off by 2 roundings at most
+__device__ __forceinline__ float inverse_sqrt(float v)
 {
-    constexpr int E = Elem<T>::E;
-    if (VEC) return (int)(((int64_t)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) + row * ldx) & (E - 1));
-    return mask.on ? (int)((mask.first + row * cols) & 3) : 0;
+    float s;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
+    return fmaf(0.5f * s, fmaf(-v * s, s, 1.f), s);
 }
 
-template <typename T, int L, int CH, bool VEC>
-__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS)
+template <typename T, int L, int CH, int LAYOUT>
+__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS, L > 0 ? (CH * Elem<T>::E <= 8 ? 3 : 2) : 1)
 layer_norm_kernel(const __grid_constant__ NormForward p)
 {
     constexpr int E = Elem<T>::E;
+    constexpr bool VEC = LAYOUT != ROWS_LOOSE;
     __shared__ GroupSums<1> s_one;
     __shared__ GroupSums<2> s_two;
     int turn_one = 0, turn_two = 0;
@@ -67,45 +139,67 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         clear_sums(s_two);
         __syncthreads();
     }
-    const int lanes = L > 0 ? L : (int)blockDim.x, t = L > 0 ? (int)threadIdx.x % (L > 0 ? L : 1) : (int)threadIdx.x;
-    const int sub = L > 0 ? ((int)threadIdx.x & 31) / (L > 0 ? L : 1) : 0;           // group within the warp
-    const int64_t groups = (int64_t)gridDim.x * (L > 0 ? NORM_THREADS / (L > 0 ? L : 1) : 1);
-    const int64_t group = L > 0 ? ((int64_t)blockIdx.x * NORM_THREADS + threadIdx.x) / (L > 0 ? L : 1) : (int64_t)blockIdx.x;
-    const int cols = p.cols, shift = row_shift<T, VEC>(p.x, p.ldx, p.mask, cols, group);
-    const int64_t offset = mask_offset(p.mask);
+    const int cols = p.cols;
+    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols, p.mask);
 
-    float w[CH][E], b[CH][E];
-    uint32_t ok = 0;                                     // which of the thread's columns there are
+    extern __shared__ uint4 s_ring[];
+    RowRing<T, 1, CH, NORM_STAGES> ring(s_ring);
+    const T *const first = static_cast<const T *>(p.x), *x = first + at.group * p.ldx + at.column(0);
+    if (VEC) {
 #pragma unroll
-    for (int j = 0; j < CH; j++) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int c = (j * lanes + t) * E - shift + e;
-            const bool in = c >= 0 && c < cols;
-            if (in) ok |= 1u << (j * E + e);
-            w[j][e] = in && p.weight != nullptr ? p.weight[c] : 1.f;
-            b[j][e] = in && p.bias != nullptr ? p.bias[c] : 0.f;
+        for (int k = 0; k < NORM_STAGES; k++) {
+            ring.clear();
+            if (k < at.turns) at.fetch(ring, 0, x, first, cols);
+            commit_copies();
+            ring.next();
+            x += p.x_step;
         }
     }
 
-    for (int64_t base = group - sub; base < p.rows; base += groups) {
-        const int64_t row = base + sub;
-        const bool live = row < p.rows;
+    float w[CH][E], b[CH][E];
+    uint32_t own[CH][E];
+#pragma unroll
+    for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int c = at.column(j) + e;
+            const bool in = c >= 0 && c < cols;
+            // the mask's factor is in them: what is kept is multiplied by it, and it is positive
+            const float scale = p.mask.on ? p.mask.scale : 1.f;
+            w[j][e] = in && p.weight != nullptr ? p.weight[c] * scale : scale;
+            b[j][e] = in && p.bias != nullptr ? p.bias[c] * scale : 0.f;
+            own[j][e] = at.mine(j, e);
+        }
+    const int64_t offset = mask_offset(p.mask);
+    const int64_t number = p.mask.first + at.group * cols - at.shift;       // of the row's first element; the same within a block in all rows
+    const int skip = (int)(number & 3);
+    int64_t block = (number >> 2) + at.t * (E / 4);
+    T *y = static_cast<T *>(p.y) + at.group * p.ldy + at.column(0);
+    float2 *stats = p.stats + at.group;
+
+    for (int k = 0; k < at.warp_turns; k++) {
+        const bool live = k < at.turns;
         float d[CH][E];
         float one[1] = {0.f}, two[2] = {0.f, 0.f};
+        if (VEC) {
+            wait_copies<NORM_STAGES - 1>();
 #pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int c0 = (j * lanes + t) * E - shift;
-            if (live && c0 < cols) load_chunk<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx, c0, cols, d[j]);
-            else {
+            for (int j = 0; j < CH; j++) ring.get(0, j, d[j]);
+            if (k + NORM_STAGES < at.turns) at.fetch(ring, 0, x, first, cols);
+            commit_copies();
+            ring.next();
+        } else {
 #pragma unroll
-                for (int e = 0; e < E; e++) d[j][e] = 0.f;
-            }
+            for (int j = 0; j < CH; j++) load_chunk<T, false>(x - at.column(0), live ? at.column(j) : cols, cols, d[j]);
         }
+        x += p.x_step;
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) one[0] += d[j][e];
+            for (int e = 0; e < E; e++) {
+                if (LAYOUT == ROWS_EDGES) d[j][e] = masked(d[j][e], own[j][e]);
+                one[0] += d[j][e];
+            }
         group_sum<L, 1>(one, s_one, turn_one);
         // The first mean is off by its own rounding; the second sum says by how much, and the squares are taken around
         // the first: nothing cancels, however far the mean is from zero.
@@ -114,152 +208,217 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         for (int j = 0; j < CH; j++)
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                d[j][e] = ok >> (j * E + e) & 1u ? d[j][e] - m : 0.f;
+                d[j][e] = LAYOUT == ROWS_WHOLE ? d[j][e] - masked(m, own[j][0]) : masked(d[j][e] - m, own[j][e]);
                 two[0] += d[j][e];
                 two[1] = fmaf(d[j][e], d[j][e], two[1]);
             }
         group_sum<L, 2>(two, s_two, turn_two);
         const float off = two[0] * p.inv_cols;
         const float var = fmaf(-off, off, two[1] * p.inv_cols);
-        const float s = __frsqrt_rn((var < 0.f ? 0.f : var) + p.eps);
-        if (!live) continue;
-        if (p.stats != nullptr && t == 0) p.stats[row] = make_float2(m + off, s);
+        const float s = inverse_sqrt(relu_of(var) + p.eps);
+        const float shifted = -off * s;
 #pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int c0 = (j * lanes + t) * E - shift;
-            if (c0 >= cols) continue;
-            float v[E];
+        for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                v[e] = fmaf((d[j][e] - off) * s, w[j][e], b[j][e]);
-                if (p.relu) v[e] = relu_of(v[e]);
-            }
-            if (p.mask.on) {
-                const uint32_t keep = keep_bits<E>(p.mask, offset, p.mask.first + row * cols + c0);
+            for (int e = 0; e < E; e++) d[j][e] = fmaf(fmaf(d[j][e], s, shifted), w[j][e], b[j][e]);
+        if (p.relu) {
 #pragma unroll
-                for (int e = 0; e < E; e++) v[e] = keep >> e & 1u ? v[e] * p.mask.scale : 0.f;
-            }
-            store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy, c0, cols, v);
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) d[j][e] = relu_of(d[j][e]);
         }
+        if (p.mask.on) {
+            uint32_t word[CH][E];
+            draw_words<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, word);
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) d[j][e] = word[j][e] >= p.mask.threshold ? d[j][e] : 0.f;
+        }
+        if (live) {
+            if (p.stats != nullptr && at.t == 0) *stats = make_float2(m + off, s);
+            at.template store<VEC>(y, cols, d);
+        }
+        y += p.y_step;
+        stats += at.groups;
+        block += p.part.words;
     }
 }
 
-template <typename T, int L, int CH, bool VEC>
-__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS)
+template <typename T, int L, int CH, int LAYOUT>
+__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS, L > 0 && CH * Elem<T>::E <= 8 ? 2 : 1)
 layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
 {
     constexpr int E = Elem<T>::E;
+    constexpr bool VEC = LAYOUT != ROWS_LOOSE;
     __shared__ GroupSums<2> s_two;
-    __shared__ float s_cols[L > 0 ? NORM_THREADS * CH * E : 1];
     int turn = 0;
     if (L == 0) {
         clear_sums(s_two);
         __syncthreads();
     }
-    const int lanes = L > 0 ? L : (int)blockDim.x, t = L > 0 ? (int)threadIdx.x % (L > 0 ? L : 1) : (int)threadIdx.x;
-    const int sub = L > 0 ? ((int)threadIdx.x & 31) / (L > 0 ? L : 1) : 0;
-    const int64_t groups = (int64_t)gridDim.x * (L > 0 ? NORM_THREADS / (L > 0 ? L : 1) : 1);
-    const int64_t group = L > 0 ? ((int64_t)blockIdx.x * NORM_THREADS + threadIdx.x) / (L > 0 ? L : 1) : (int64_t)blockIdx.x;
-    const int cols = p.cols, shift = row_shift<T, VEC>(p.x, p.ldx, p.mask, cols, group);
-    const int64_t offset = mask_offset(p.mask);
+    const int cols = p.cols;
+    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols, p.mask);
+
+    extern __shared__ uint4 s_ring[];
+    RowRing<T, 2, CH, NORM_STAGES> ring(s_ring);
+    const T *const x_first = static_cast<const T *>(p.x), *const dy_first = static_cast<const T *>(p.dy);
+    const T *x = x_first + at.group * p.ldx + at.column(0), *dy = dy_first + at.group * p.lddy + at.column(0);
+    if (VEC) {
+#pragma unroll
+        for (int k = 0; k < NORM_STAGES; k++) {
+            ring.clear();
+            if (k < at.turns) {
+                at.fetch(ring, 0, x, x_first, cols);
+                at.fetch(ring, 1, dy, dy_first, cols);
+            }
+            commit_copies();
+            ring.next();
+            x += p.x_step;
+            dy += p.dy_step;
+        }
+    }
 
     float w[CH][E], b[CH][E], sum_w[CH][E], sum_b[CH][E];
-    uint32_t ok = 0;
+    uint32_t own[CH][E];
+    float uncertain = 0.f;
 #pragma unroll
-    for (int j = 0; j < CH; j++) {
+    for (int j = 0; j < CH; j++)
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int c = (j * lanes + t) * E - shift + e;
+            const int c = at.column(j) + e;
             const bool in = c >= 0 && c < cols;
-            if (in) ok |= 1u << (j * E + e);
             w[j][e] = in && p.weight != nullptr ? p.weight[c] : 1.f;
-            b[j][e] = in && p.bias != nullptr ? p.bias[c] : 0.f;
+            b[j][e] = !in ? INFINITY : p.bias != nullptr ? p.bias[c] : 0.f;       // a column that is not there is never near zero
+            // z = h w + b is off by less than 2^-22 |b| where the two terms cancel: its sign is not certain below that
+            if (in) uncertain = fmaxf(uncertain, fabsf(b[j][e]) * 4.76837158e-7f);
             sum_w[j][e] = sum_b[j][e] = 0.f;
+            own[j][e] = at.mine(j, e);
         }
-    }
+    const float scale = p.mask.on ? p.mask.scale : 1.f;       // of all gradients: once per row and at the end
+    const int64_t offset = mask_offset(p.mask);
+    const int64_t number = p.mask.first + at.group * cols - at.shift;
+    const int skip = (int)(number & 3);
+    int64_t block = (number >> 2) + at.t * (E / 4);
+    T *dx = static_cast<T *>(p.dx) + at.group * p.lddx + at.column(0);
+    const float2 *stats_at = p.stats + at.group;
+    float2 next_stats = at.turns > 0 ? *stats_at : make_float2(0.f, 0.f);
 
-    for (int64_t base = group - sub; base < p.rows; base += groups) {
-        const int64_t row = base + sub;
-        const bool live = row < p.rows;
+    for (int k = 0; k < at.warp_turns; k++) {
+        const bool live = k < at.turns;
         float h[CH][E], g[CH][E];
         float two[2] = {0.f, 0.f};
-        const float2 stats = live ? p.stats[row] : make_float2(0.f, 0.f);
+        const float2 stats = next_stats;
+        stats_at += at.groups;
+        if (k + 1 < at.turns) next_stats = *stats_at;
+        if (VEC) {
+            wait_copies<NORM_STAGES - 1>();
 #pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int c0 = (j * lanes + t) * E - shift;
-            if (live && c0 < cols) {
-                load_chunk<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx, c0, cols, h[j]);
-                load_chunk<T, VEC>(static_cast<const T *>(p.dy) + row * p.lddy, c0, cols, g[j]);
-            } else {
+            for (int j = 0; j < CH; j++) {
+                ring.get(0, j, h[j]);
+                ring.get(1, j, g[j]);
+            }
+            if (k + NORM_STAGES < at.turns) {
+                at.fetch(ring, 0, x, x_first, cols);
+                at.fetch(ring, 1, dy, dy_first, cols);
+            }
+            commit_copies();
+            ring.next();
+        } else {
 #pragma unroll
-                for (int e = 0; e < E; e++) h[j][e] = g[j][e] = 0.f;
+            for (int j = 0; j < CH; j++) {
+                load_chunk<T, false>(x - at.column(0), live ? at.column(j) : cols, cols, h[j]);
+                load_chunk<T, false>(dy - at.column(0), live ? at.column(j) : cols, cols, g[j]);
             }
         }
 #pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int c0 = (j * lanes + t) * E - shift;
-            const uint32_t keep = p.mask.on && live && c0 < cols ? keep_bits<E>(p.mask, offset, p.mask.first + row * cols + c0) : ~0u;
-            bool near = false;
-            uint32_t pass = ~0u;
+        for (int j = 0; j < CH; j++)
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const float x = h[j][e];
-                h[j][e] = ok >> (j * E + e) & 1u ? (x - stats.x) * stats.y : 0.f;
-                if (p.relu) {
-                    const float z = fmaf(h[j][e], w[j][e], b[j][e]);
-                    if (!relu_passes(z)) pass &= ~(1u << e);
-                    // |z| off by less than 2^-22 |b| where the two terms cancel: the sign is not certain below that
-                    near = near || fabsf(z) < 4.76837158e-7f * fabsf(b[j][e]);
+                // what else a slot holds does not count
+                if (LAYOUT == ROWS_WHOLE) {
+                    h[j][e] = (h[j][e] - masked(stats.x, own[j][0])) * stats.y;
+                } else {
+                    h[j][e] = masked((h[j][e] - stats.x) * stats.y, own[j][e]);
+                    g[j][e] = masked(g[j][e], own[j][e]);
                 }
             }
-            if (near) {
+        if (p.relu) {
+            bool near = false;
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float z = fmaf(h[j][e], w[j][e], b[j][e]);
+                    near = near || fabsf(z) < uncertain;
+                    g[j][e] = relu_passes(z) ? g[j][e] : 0.f;
+                }
+            if (near && live) {
                 // One element in millions: in 64 bits, so that a gradient passes where the formula lets it pass.
-                float x[E];
-                load_chunk<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx, c0, cols, x);
-                pass = ~0u;
+                const int ahead = VEC ? NORM_STAGES : 0;
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (((double)x[e] - (double)stats.x) * (double)stats.y * (double)w[j][e] + (double)b[j][e] <= 0.0) pass &= ~(1u << e);
-            }
+                for (int j = 0; j < CH; j++) {
+                    load_chunk<T, false>(x - ahead * p.x_step - at.column(0), at.column(j), cols, h[j]);
+                    load_chunk<T, false>(dy - ahead * p.dy_step - at.column(0), at.column(j), cols, g[j]);
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                float dz = g[j][e];
-                if (p.mask.on) dz *= p.mask.scale;
-                dz = (keep & pass) >> e & 1u ? dz : 0.f;
-                sum_w[j][e] = fmaf(dz, h[j][e], sum_w[j][e]);
-                sum_b[j][e] += dz;
-                g[j][e] = dz * w[j][e];
-                two[0] += g[j][e];
-                two[1] = fmaf(g[j][e], h[j][e], two[1]);
+                    for (int e = 0; e < E; e++) {
+                        const double d = (double)h[j][e] - (double)stats.x;
+                        if (d * (double)stats.y * (double)w[j][e] + (double)b[j][e] <= 0.0) g[j][e] = 0.f;
+                        h[j][e] = at.ok >> (j * E + e) & 1u ? (h[j][e] - stats.x) * stats.y : 0.f;
+                    }
+                }
             }
+        }
+        x += p.x_step;
+        dy += p.dy_step;
+        if (p.mask.on) {
+            uint32_t word[CH][E];
+            draw_words<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, word);
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) g[j][e] = word[j][e] >= p.mask.threshold ? g[j][e] : 0.f;
+        }
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    sum_w[j][e] = fmaf(g[j][e], h[j][e], sum_w[j][e]);
+                    sum_b[j][e] += g[j][e];
+                    g[j][e] *= w[j][e];
+                    two[0] += g[j][e];
+                    two[1] = fmaf(g[j][e], h[j][e], two[1]);
+                }
         }
         group_sum<L, 2>(two, s_two, turn);
-        if (!live) continue;
-        const float m1 = two[0] * p.inv_cols, m2 = two[1] * p.inv_cols;
+        if (live) {
+            const float s = stats.y * scale, m1 = two[0] * p.inv_cols * s, m2 = two[1] * p.inv_cols * s;
 #pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int c0 = (j * lanes + t) * E - shift;
-            if (c0 >= cols) continue;
-            float v[E];
+            for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = stats.y * (g[j][e] - m1 - h[j][e] * m2);
-            store_chunk<T, VEC>(static_cast<T *>(p.dx) + row * p.lddx, c0, cols, v);
+                for (int e = 0; e < E; e++) g[j][e] = fmaf(-h[j][e], m2, fmaf(g[j][e], s, -m1));
+            at.template store<VEC>(dx, cols, g);
         }
+        dx += p.dx_step;
+        block += p.part.words;
     }
 
+    if (VEC) wait_copies<0>();
     // The groups' sums, then the thread blocks': always in the same order.
 #pragma unroll
     for (int pass = 0; pass < 2; pass++) {
         float *part = pass == 0 ? p.dweight : p.dbias;
         if (part == nullptr) continue;
         part += (int64_t)blockIdx.x * p.part_stride;
+        float *s_cols = reinterpret_cast<float *>(s_ring);       // the ring is empty by now
         if (L > 0) __syncthreads();
         float *mine = L > 0 ? s_cols + (threadIdx.x / (L > 0 ? L : 1)) * cols : part;
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (ok >> (j * E + e) & 1u) mine[(j * lanes + t) * E - shift + e] = pass == 0 ? sum_w[j][e] : sum_b[j][e];
+                if (at.ok >> (j * E + e) & 1u) mine[at.column(j) + e] = (pass == 0 ? sum_w[j][e] : sum_b[j][e]) * scale;
         if (L > 0) {
             __syncthreads();
             for (int c = threadIdx.x; c < cols; c += NORM_THREADS) {

@@ -9,50 +9,73 @@ namespace agcn {
 
 // What a kernel needs to make its part of a mask again.
 struct DropoutMask {
-    int on;                       // 0: everything is kept, unscaled
-    uint32_t key0, key1;          // seed
-    uint32_t threshold;           // floor(p 2^32)
-    float scale;                  // 1 / (1 - p)
+    int on;                                // 0: everything is kept, unscaled
+    uint32_t key0, key1;                   // seed
+    uint32_t threshold;                    // floor(p 2^32)
+    float scale;                           // 1 / (1 - p)
     int64_t offset;
-    const int64_t *step;          // added to offset, read when the kernel runs (null: 0)
-    int64_t first;                // number of the first element: row0 * cols
+    const int64_t *step;                   // added to offset, read when the kernel runs (null: 0)
+    int64_t first;                         // number of the first element: row0 * cols
 };
 
-// Four words: two 32 x 32 -> 64 bit products, four exclusive ors and two key additions per round, ten rounds.
-__device__ __forceinline__ uint4 philox4x32(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1)
+// The words of N blocks side by side: two 32 x 32 -> 64 bit products and two three-way exclusive ors a round and block; the
+// two additions that make a round's keys serve all N.
+template <int N>
+__device__ __forceinline__ void philox4x32(const DropoutMask &m, int64_t offset, const int64_t (&block)[N], uint32_t (&w)[N][4])
 {
+    uint32_t k0 = m.key0, k1 = m.key1;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        w[n][0] = (uint32_t)block[n]; w[n][1] = (uint32_t)((uint64_t)block[n] >> 32);
+        w[n][2] = (uint32_t)offset; w[n][3] = (uint32_t)((uint64_t)offset >> 32);
+    }
 #pragma unroll
     for (int round = 0; round < 10; round++) {
-        const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-        c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
-        c3 = (uint32_t)a;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const uint64_t a = (uint64_t)w[n][0] * 0xD2511F53u, b = (uint64_t)w[n][2] * 0xCD9E8D57u;
+            w[n][0] = (uint32_t)(b >> 32) ^ w[n][1] ^ k0;
+            w[n][1] = (uint32_t)b;
+            w[n][2] = (uint32_t)(a >> 32) ^ w[n][3] ^ k1;
+            w[n][3] = (uint32_t)a;
+        }
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
-    return make_uint4(c0, c1, c2, c3);
 }
 
-// Bit e: whether word e of block `block` keeps its element.
-__device__ __forceinline__ uint32_t keep_block(const DropoutMask &m, int64_t offset, int64_t block)
+// Words of CH chunks of E elements; chunk j begins with word `skip` (0 to 3, alike for all) of block `block` + j * stride.
+// Element e is kept if its word is at least m.threshold.  (Where the chunks do not begin with a block, a word stands for
+// the answer: 0, or all ones.)
+template <int CH, int E>
+__device__ __forceinline__ void draw_words(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, uint32_t (&word)[CH][E])
 {
-    const uint4 w = philox4x32((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32), m.key0, m.key1);
-    return (w.x >= m.threshold ? 1u : 0u) | (w.y >= m.threshold ? 2u : 0u) | (w.z >= m.threshold ? 4u : 0u) | (w.w >= m.threshold ? 8u : 0u);
-}
-
-// Bits 0 .. E - 1: whether elements i, i + 1, ... are kept (E a multiple of 4; elements before the first one, i < 0, may
-// be asked for and mean nothing).
-template <int E>
-__device__ __forceinline__ uint32_t keep_bits(const DropoutMask &m, int64_t offset, int64_t i)
-{
-    const int64_t block = i >> 2;
-    const int skip = (int)(i & 3);
-    uint32_t bits = 0;
+    constexpr int B = E / 4;
+    int64_t blocks[CH * B];
+    uint32_t w[CH * B][4];
 #pragma unroll
-    for (int k = 0; k < E / 4; k++) bits |= keep_block(m, offset, block + k) << (4 * k);
-    if (skip != 0) bits = (bits | keep_block(m, offset, block + E / 4) << E) >> skip;
-    return bits;
+    for (int n = 0; n < CH * B; n++) blocks[n] = block + (n / B) * stride + n % B;
+    philox4x32<CH * B>(m, offset, blocks, w);
+#pragma unroll
+    for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) word[j][e] = w[j * B + e / 4][e % 4];
+    if (skip != 0) {
+        int64_t more[CH];
+        uint32_t v[CH][4];
+#pragma unroll
+        for (int j = 0; j < CH; j++) more[j] = block + j * stride + B;
+        philox4x32<CH>(m, offset, more, v);
+#pragma unroll
+        for (int j = 0; j < CH; j++) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int e = 0; e < E + 4; e++) bits |= ((e < E ? word[j][e < E ? e : 0] : v[j][e < E ? 0 : e - E]) >= m.threshold ? 1u : 0u) << e;
+            bits >>= skip;
+#pragma unroll
+            for (int e = 0; e < E; e++) word[j][e] = bits >> e & 1u ? ~0u : 0u;       // threshold > 0 wherever an element may be dropped
+        }
+    }
 }
 
 __device__ __forceinline__ int64_t mask_offset(const DropoutMask &m) { return m.on && m.step != nullptr ? m.offset + *m.step : m.offset; }

@@ -81,20 +81,87 @@ __device__ __forceinline__ void load_chunk(const T *row, int c0, int cols, float
         for (int e = 0; e < E; e++) v[e] = c0 + e >= 0 && c0 + e < cols ? Elem<T>::get(row[c0 + e]) : 0.f;
     }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_chunk(T *row, int c0, int cols, const float *v)
+// The same into memory; `to`: where column c0 goes (in front of the row for c0 < 0).  WHOLE: the chunk is known to be whole.
+template <typename T, bool VEC, bool WHOLE>
+__device__ __forceinline__ void store_chunk(T *to, int c0, int cols, const float *v)
 {
     constexpr int E = Elem<T>::E;
-    if (VEC && c0 >= 0 && c0 + E <= cols) {
-        *reinterpret_cast<uint4 *>(row + c0) = Elem<T>::pack(v);
+    if (VEC && (WHOLE || (c0 >= 0 && c0 + E <= cols))) {
+        *reinterpret_cast<uint4 *>(to) = Elem<T>::pack(v);
     } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) if (c0 + e >= 0 && c0 + e < cols) row[c0 + e] = Elem<T>::put(v[e]);
+        for (int e = 0; e < E; e++) if (c0 + e >= 0 && c0 + e < cols) to[e] = Elem<T>::put(v[e]);
     }
 }
 
+// 16 bytes from global to shared memory behind the thread's back; what is past `bytes` becomes 0 and is not read.
+__device__ __forceinline__ void copy_chunk(uint32_t to, const void *from, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_chunk(uint32_t to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most N of the thread's groups of copies are under way
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ uint4 load_shared(uint32_t from)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_shared(uint32_t to, const uint4 &v)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" :: "r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A thread's ring of rows that are under way from memory: STAGES rows ahead, N tensors, CH chunks each.  A slot belongs to
+// one thread, which fills and reads it: nothing to synchronise.  Registers hold the row that is worked on and nothing
+// else, and the bytes in flight do not depend on how many threads fit an SM.
+template <typename T, int N, int CH, int STAGES>
+struct RowRing {
+    uint32_t at, begin, slots;           // this thread's place in the stage that is read next, and in the first; bytes between two slots
+    __device__ __forceinline__ RowRing(void *s) : at((uint32_t)__cvta_generic_to_shared(s) + threadIdx.x * 16u), begin(at), slots(blockDim.x * 16u) {}
+    __device__ __forceinline__ uint32_t slot(int k, int j) const { return at + (k * CH + j) * slots; }
+    __device__ __forceinline__ void next()
+    {
+        at += N * CH * slots;
+        if (at == begin + STAGES * N * CH * slots) at = begin;
+    }
+    __device__ __forceinline__ void clear() const
+    {
+#pragma unroll
+        for (int k = 0; k < N * CH; k++) store_shared(at + k * slots, make_uint4(0, 0, 0, 0));
+    }
+    // Starts the copy of chunk j of tensor k: of a whole one at `from`, ...
+    __device__ __forceinline__ void fetch(int k, int j, const T *from) const { copy_chunk(slot(k, j), from); }
+    // ... or of `bytes` of it, elements c0 .. of a row: what is in front of the row within its first 16 bytes comes along, unused;
+    // nothing in front of the tensor, at `first`, or behind the row is read.
+    __device__ __forceinline__ void fetch_edge(int k, int j, const T *from, const T *first, int c0, int cols, int bytes) const
+    {
+        if (from < first) {
+            float v[Elem<T>::E];
+            load_chunk<T, false>(from - c0, c0, cols, v);
+            store_shared(slot(k, j), Elem<T>::pack(v));
+        } else {
+            copy_chunk(slot(k, j), from, bytes);
+        }
+    }
+    __device__ __forceinline__ void get(int k, int j, float *v) const { Elem<T>::unpack(load_shared(slot(k, j)), v); }
+};
+
+__device__ __forceinline__ float masked(float v, uint32_t bits) { return __uint_as_float(__float_as_uint(v) & bits); }
+
 // max(v, 0) that lets NaN through, and whether a gradient passes
-__device__ __forceinline__ float relu_of(float v) { return v < 0.f ? 0.f : v; }
+__device__ __forceinline__ float relu_of(float v)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ bool relu_passes(float v) { return !(v <= 0.f); }
 
 // Sums of K values over a group of L lanes of a warp, or (L = 0) over the thread block; every thread gets them, added

@@ -7,31 +7,37 @@ namespace agcn {
 
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
+constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
+constexpr int NORM_MAX_SMEM = NORM_STAGES * 2 * NORM_ELEMS * 4 * NORM_MAX_THREADS;
 
 struct NormForm {
-    bool vec;
+    int layout;                             // RowLayout
     int lanes;                              // per row; 0: a thread block of `threads`
     int chunks;                             // of 16 bytes per lane
     int threads;
     int64_t rows_per_block;
 };
 
-inline NormForm norm_form(const Rows *t, int n, int64_t cols, int dtype, bool mask)
+// `per_lane`: elements of a row per lane of a group within a warp that are aimed at
+inline NormForm norm_form(const Rows *t, int n, int64_t cols, int dtype, bool mask, int per_lane)
 {
     const int e = 16 / dtype_bytes(dtype), most_chunks = NORM_ELEMS / e;
     NormForm f = {};
     int shift = 0;
-    f.vec = rows_sit_alike(t, n, dtype, &shift);
-    if (!f.vec) shift = mask ? 3 : 0;
+    f.layout = !rows_sit_alike(t, n, dtype, &shift) ? ROWS_LOOSE : shift != 0 || cols % e != 0 ? ROWS_EDGES : ROWS_WHOLE;
+    if (f.layout == ROWS_LOOSE) shift = mask ? 3 : 0;
     const int chunks = (int)ceil_div(cols + shift, e);
-    f.lanes = 4;
-    while (f.lanes <= 32 && f.lanes * most_chunks < chunks) f.lanes *= 2;
+    f.lanes = 2;
+    while (f.lanes < 32 && f.lanes * per_lane / e < chunks) f.lanes *= 2;
     f.threads = NORM_THREADS;
-    if (f.lanes > 32) {
+    f.chunks = (int)ceil_div(chunks, f.lanes);
+    if (f.chunks > most_chunks) {
         f.lanes = 0;
+        f.chunks = most_chunks;
         f.threads = 32 * (int)ceil_div(chunks, 32 * most_chunks);
+    } else if (f.chunks == 3) {
+        f.chunks = 4;
     }
-    f.chunks = f.vec && f.lanes > 0 ? (int)ceil_div(chunks, f.lanes) : most_chunks;
     f.rows_per_block = f.lanes > 0 ? NORM_THREADS / f.lanes : 1;
     return f;
 }
@@ -44,45 +50,63 @@ inline int64_t norm_grid(const NormForm &f, int64_t rows, int64_t resident)
     return needed < resident ? needed : resident;
 }
 
-// Calls launch.template operator()<T, L, CH, VEC>() of the form.
-template <typename T, bool VEC, int L, typename F> int norm_dispatch_chunks(const NormForm &f, F &&launch)
+// Calls launch.template operator()<T, L, CH, LAYOUT>() of the form.
+template <typename T, int LAYOUT, int L, typename F> int norm_dispatch_chunks(const NormForm &f, F &&launch)
 {
     constexpr int MOST = NORM_ELEMS / Elem<T>::E;
-    if constexpr (VEC && L > 0) {
-        if (f.chunks == 1) return launch.template operator()<T, L, 1, VEC>();
-        if constexpr (MOST == 4) {
-            if (f.chunks == 2) return launch.template operator()<T, L, 2, VEC>();
-            if (f.chunks == 3) return launch.template operator()<T, L, 3, VEC>();
-        }
+    if constexpr (L > 0) {
+        if (f.chunks == 1) return launch.template operator()<T, L, 1, LAYOUT>();
+        if constexpr (MOST == 4) if (f.chunks == 2) return launch.template operator()<T, L, 2, LAYOUT>();
     }
-    return launch.template operator()<T, L, MOST, VEC>();
+    return launch.template operator()<T, L, MOST, LAYOUT>();
 }
-template <typename T, bool VEC, typename F> int norm_dispatch_lanes(const NormForm &f, F &&launch)
+template <typename T, int LAYOUT, typename F> int norm_dispatch_lanes(const NormForm &f, F &&launch)
 {
     switch (f.lanes) {
-    case 4: return norm_dispatch_chunks<T, VEC, 4>(f, launch);
-    case 8: return norm_dispatch_chunks<T, VEC, 8>(f, launch);
-    case 16: return norm_dispatch_chunks<T, VEC, 16>(f, launch);
-    case 32: return norm_dispatch_chunks<T, VEC, 32>(f, launch);
-    default: return norm_dispatch_chunks<T, VEC, 0>(f, launch);
+    case 2: return norm_dispatch_chunks<T, LAYOUT, 2>(f, launch);
+    case 4: return norm_dispatch_chunks<T, LAYOUT, 4>(f, launch);
+    case 8: return norm_dispatch_chunks<T, LAYOUT, 8>(f, launch);
+    case 16: return norm_dispatch_chunks<T, LAYOUT, 16>(f, launch);
+    case 32: return norm_dispatch_chunks<T, LAYOUT, 32>(f, launch);
+    default: return norm_dispatch_chunks<T, LAYOUT, 0>(f, launch);
     }
+}
+template <typename T, typename F> int norm_dispatch_layout(const NormForm &f, F &&launch)
+{
+    if (f.layout == ROWS_WHOLE) return norm_dispatch_lanes<T, ROWS_WHOLE>(f, launch);
+    return f.layout == ROWS_EDGES ? norm_dispatch_lanes<T, ROWS_EDGES>(f, launch) : norm_dispatch_lanes<T, ROWS_LOOSE>(f, launch);
 }
 template <typename F> int norm_dispatch(const NormForm &f, int dtype, F &&launch)
 {
-    if (dtype == AGCN_F32) return f.vec ? norm_dispatch_lanes<float, true>(f, launch) : norm_dispatch_lanes<float, false>(f, launch);
-    if (dtype == AGCN_BF16) return f.vec ? norm_dispatch_lanes<__nv_bfloat16, true>(f, launch) : norm_dispatch_lanes<__nv_bfloat16, false>(f, launch);
-    return f.vec ? norm_dispatch_lanes<__half, true>(f, launch) : norm_dispatch_lanes<__half, false>(f, launch);
+    if (dtype == AGCN_F32) return norm_dispatch_layout<float>(f, launch);
+    return dtype == AGCN_BF16 ? norm_dispatch_layout<__nv_bfloat16>(f, launch) : norm_dispatch_layout<__half>(f, launch);
+}
+
+// Dynamic shared memory: the ring of `tensors` tensors, and at the end the groups' column sums
+inline int norm_smem(const NormForm &f, int tensors) { return NORM_STAGES * tensors * f.chunks * f.threads * 16; }
+
+inline NormRows norm_rows(const NormForm &f, int64_t grid, int64_t rows, int64_t cols, int64_t *groups)
+{
+    *groups = grid * f.rows_per_block;
+    NormRows r = {};
+    r.turns = (int)(rows / *groups);
+    r.rest = rows % *groups;
+    r.words = *groups * cols / 4;          // whole wherever a group has a second row: *groups is a multiple of 8 then
+    return r;
 }
 
 // Thread blocks of a kernel that the current device holds at once, asked for once per device and block size
-template <auto KERNEL> int norm_resident(int threads, int64_t *blocks)
+template <auto KERNEL> int norm_resident(int threads, int smem, int64_t *blocks)
 {
     static int per_sm[64][ROW_WARPS + 1] = {};
     int dev = 0, sms = 0;
     const int rc = current_sm_count(&dev, &sms);
     if (rc != AGCN_OK) return rc;
     int &n = per_sm[dev][threads / 32];
-    if (n == 0) AGCN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0));
+    if (n == 0) {
+        AGCN_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_MAX_SMEM));
+        AGCN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem));
+    }
     *blocks = (int64_t)n * sms;
     return AGCN_OK;
 }
