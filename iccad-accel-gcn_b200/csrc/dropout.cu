@@ -5,19 +5,47 @@
 
 namespace agcn {
 
-template <typename T, bool VEC>
-static int dropout_launch(DropoutParams &p, cudaStream_t s)
+// Thread blocks of a kernel that the current device holds at once
+template <auto KERNEL> static int dropout_resident(int64_t *blocks)
 {
+    static int per_sm[64] = {};
     int dev = 0, sms = 0;
     const int rc = current_sm_count(&dev, &sms);
     if (rc != AGCN_OK) return rc;
-    const int64_t chunks = ceil_div(p.cols, Elem<T>::E);
+    if (per_sm[dev] == 0) AGCN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[dev], KERNEL, DROPOUT_THREADS, 0));
+    *blocks = (int64_t)per_sm[dev] * sms;
+    return AGCN_OK;
+}
+
+template <auto KERNEL> static int dropout_start(const DropoutParams &p, int64_t threads, cudaStream_t s)
+{
+    int64_t resident = 0;
+    const int rc = dropout_resident<KERNEL>(&resident);
+    if (rc != AGCN_OK) return rc;
+    const int64_t needed = ceil_div(threads, DROPOUT_THREADS);
+    resident = resident / 8 * 8;
+    KERNEL<<<(unsigned)(needed < resident ? needed : resident), DROPOUT_THREADS, 0, s>>>(p);
+    AGCN_LAUNCH_CHECK("dropout kernel");
+    return AGCN_OK;
+}
+
+template <typename T, bool GATE>
+static int dropout_launch(DropoutParams &p, bool array, int layout, int shift, cudaStream_t s)
+{
+    if (array) return dropout_start<dropout_array_kernel<T, GATE>>(p, p.rows * p.cols / Elem<T>::E + 2, s);
+    const int64_t chunks = ceil_div(p.cols + shift, Elem<T>::E);
     p.lanes = 1;
     while (p.lanes < DROPOUT_THREADS && p.lanes < chunks) p.lanes *= 2;
-    const int64_t needed = ceil_div(p.rows * p.lanes, DROPOUT_THREADS), most = (int64_t)sms * 8;
-    dropout_kernel<T, VEC><<<(unsigned)(needed < most ? needed : most), DROPOUT_THREADS, 0, s>>>(p);
-    AGCN_LAUNCH_CHECK("dropout_kernel");
-    return AGCN_OK;
+    const int64_t threads = p.rows * p.lanes;
+    if (layout == ROWS_WHOLE) return dropout_start<dropout_rows_kernel<T, ROWS_WHOLE, GATE>>(p, threads, s);
+    return layout == ROWS_EDGES ? dropout_start<dropout_rows_kernel<T, ROWS_EDGES, GATE>>(p, threads, s)
+                                : dropout_start<dropout_rows_kernel<T, ROWS_LOOSE, GATE>>(p, threads, s);
+}
+
+template <typename T>
+static int dropout_typed(DropoutParams &p, bool array, int layout, int shift, cudaStream_t s)
+{
+    return p.gate != nullptr ? dropout_launch<T, true>(p, array, layout, shift, s) : dropout_launch<T, false>(p, array, layout, shift, s);
 }
 
 static int dropout_run(const char *who, const Rows &v, const Rows &gate, const Rows &out, int64_t rows, int64_t cols, int dtype, int activation,
@@ -37,10 +65,11 @@ static int dropout_run(const char *who, const Rows &v, const Rows &gate, const R
     a.rows = rows; a.cols = cols;
     a.relu = !backward && activation == AGCN_ACT_RELU;
     int shift = 0;
-    const bool vec = rows_sit_alike(t, n, dtype, &shift);
-    if (dtype == AGCN_F32) return vec ? dropout_launch<float, true>(a, s) : dropout_launch<float, false>(a, s);
-    if (dtype == AGCN_BF16) return vec ? dropout_launch<__nv_bfloat16, true>(a, s) : dropout_launch<__nv_bfloat16, false>(a, s);
-    return vec ? dropout_launch<__half, true>(a, s) : dropout_launch<__half, false>(a, s);
+    const int layout = rows_layout(t, n, cols, dtype, &shift);
+    bool array = layout != ROWS_LOOSE;
+    for (int k = 0; k < n; k++) array = array && (t[k].ld == cols || rows == 1);
+    if (dtype == AGCN_F32) return dropout_typed<float>(a, array, layout, shift, s);
+    return dtype == AGCN_BF16 ? dropout_typed<__nv_bfloat16>(a, array, layout, shift, s) : dropout_typed<__half>(a, array, layout, shift, s);
 }
 
 }  // namespace agcn

@@ -18,8 +18,10 @@
 namespace agcn {
 
 constexpr int NORM_STAGES = 3;             // rows ahead in the ring
+// of the backward pass, one row per thread block: two tensors of 8192 columns and the weights are 192 KB in 32 bits, 160 KB in 16
+__host__ __device__ constexpr int norm_backward_stages(int lanes, int elem) { return lanes == 0 && elem == 4 ? 2 : NORM_STAGES; }
 constexpr int NORM_THREADS = 256;          // of the forms with several rows per thread block
-constexpr int NORM_MAX_THREADS = 544;      // of the form with one: 8192 columns, 16 per thread, from any offset on
+constexpr int NORM_MAX_THREADS = 512;      // of the form with one: 8192 columns, 16 per thread
 static_assert(NORM_MAX_THREADS <= 32 * ROW_WARPS, "group_sum holds the sums of that many warps");
 
 // The rows of a call over the groups: every group has `turns` of them, the first `rest` groups one more.
@@ -57,11 +59,6 @@ struct NormBackward {
     DropoutMask mask;
 };
 
-// How the rows of all tensors of a call sit: alike with respect to 16-byte boundaries, every row beginning and ending on
-// one (WHOLE); alike, with chunks at the rows' ends that are not the row's alone (EDGES); or not alike (LOOSE: read
-// element by element).
-enum RowLayout { ROWS_WHOLE, ROWS_EDGES, ROWS_LOOSE };
-
 // Where a thread of a layer norm kernel stands.
 template <typename T, int L, int CH, int LAYOUT>
 struct NormPlace {
@@ -69,9 +66,9 @@ struct NormPlace {
     int lanes, t;                        // threads of the group, this one's number
     int64_t group, groups;
     int turns, warp_turns;               // rows of the group; the most that a group of this warp has
-    int shift;                           // elements that the group's rows begin behind a boundary: of 16 bytes, or (LOOSE) of the mask's blocks
+    int shift;                           // elements that the group's rows begin behind a 16-byte boundary (LOOSE: taken as 0)
     uint32_t ok;                         // which of the thread's CH * E columns there are
-    __device__ __forceinline__ NormPlace(const NormRows &part, const void *x, int64_t ldx, int cols, const DropoutMask &mask)
+    __device__ __forceinline__ NormPlace(const NormRows &part, const void *x, int64_t ldx, int cols)
     {
         lanes = L > 0 ? L : (int)blockDim.x;
         t = L > 0 ? (int)threadIdx.x & (L - 1) : (int)threadIdx.x;
@@ -81,7 +78,6 @@ struct NormPlace {
         warp_turns = L > 0 ? part.turns + (group - ((int)threadIdx.x & 31) / (L > 0 ? L : 1) < part.rest) : turns;
         shift = 0;
         if (LAYOUT == ROWS_EDGES) shift = (int)(((int64_t)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) + group * ldx) & (E - 1));
-        if (LAYOUT == ROWS_LOOSE && mask.on) shift = (int)((mask.first + group * cols) & 3);
         ok = 0;
 #pragma unroll
         for (int j = 0; j < CH; j++)
@@ -117,12 +113,61 @@ struct NormPlace {
     }
 };
 
+// One number per column of the thread's: in registers, or (L = 0, where the row's 16 elements per thread take those) in shared
+// memory, 16 bytes at a time: quarter q of chunk j at [j][q][thread].
+template <bool SHARED, int CH, int E>
+struct NormColumns {
+    float v[SHARED ? 1 : CH][E];
+    float4 *s;
+    int threads;
+    __device__ __forceinline__ NormColumns(void *memory) : s(static_cast<float4 *>(memory) + threadIdx.x), threads(blockDim.x) {}
+    __device__ __forceinline__ void put(int j, const float (&c)[E])
+    {
+#pragma unroll
+        for (int e = 0; e < E; e++) if (!SHARED) v[SHARED ? 0 : j][e] = c[e];
+#pragma unroll
+        for (int q = 0; q < E / 4; q++) if (SHARED) s[(j * (E / 4) + q) * threads] = make_float4(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]);
+    }
+    __device__ __forceinline__ void get(int j, float (&c)[E]) const
+    {
+#pragma unroll
+        for (int e = 0; e < E; e++) if (!SHARED) c[e] = v[SHARED ? 0 : j][e];
+#pragma unroll
+        for (int q = 0; q < E / 4; q++)
+            if (SHARED) {
+                const float4 f = s[(j * (E / 4) + q) * threads];
+                c[4 * q] = f.x; c[4 * q + 1] = f.y; c[4 * q + 2] = f.z; c[4 * q + 3] = f.w;
+            }
+    }
+};
+
 // 1 / sqrt(v): the approximation and one step of Newton's method, off by 2 roundings at most
 __device__ __forceinline__ float inverse_sqrt(float v)
 {
     float s;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(v));
     return fmaf(0.5f * s, fmaf(-v * s, s, 1.f), s);
+}
+
+// Zeroes what the mask drops of a thread's chunks; the first begins in block `block`, the next `stride` blocks later.
+template <int CH, int E>
+__device__ __forceinline__ void drop(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, float (&v)[CH][E])
+{
+    int64_t blocks[CH];
+    uint32_t word[CH][E];
+#pragma unroll
+    for (int j = 0; j < CH; j++) blocks[j] = block + j * stride;
+    draw_words<CH, E>(m, offset, blocks, skip, word);
+#pragma unroll
+    for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++) v[j][e] = word[j][e] >= m.threshold ? v[j][e] : 0.f;
+}
+
+__device__ __forceinline__ float sum4(const float2 (&v)[2])
+{
+    const float2 s = add2(v[0], v[1]);
+    return s.x + s.y;
 }
 
 template <typename T, int L, int CH, int LAYOUT>
@@ -140,7 +185,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         __syncthreads();
     }
     const int cols = p.cols;
-    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols, p.mask);
+    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols);
 
     extern __shared__ uint4 s_ring[];
     RowRing<T, 1, CH, NORM_STAGES> ring(s_ring);
@@ -180,7 +225,8 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
     for (int k = 0; k < at.warp_turns; k++) {
         const bool live = k < at.turns;
         float d[CH][E];
-        float one[1] = {0.f}, two[2] = {0.f, 0.f};
+        float one[1], two[2];
+        float2 part[3][2] = {};
         if (VEC) {
             wait_copies<NORM_STAGES - 1>();
 #pragma unroll
@@ -196,10 +242,14 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                if (LAYOUT == ROWS_EDGES) d[j][e] = masked(d[j][e], own[j][e]);
-                one[0] += d[j][e];
+            for (int e = 0; e < E; e += 2) {
+                if (LAYOUT == ROWS_EDGES && j == 0) {             // in front of the row; what is behind it is 0
+                    d[j][e] = masked(d[j][e], own[j][e]);
+                    d[j][e + 1] = masked(d[j][e + 1], own[j][e + 1]);
+                }
+                part[0][e / 2 % 2] = add2(part[0][e / 2 % 2], pair(&d[j][e]));
             }
+        one[0] = sum4(part[0]);
         group_sum<L, 1>(one, s_one, turn_one);
         // The first mean is off by its own rounding; the second sum says by how much, and the squares are taken around
         // the first: nothing cancels, however far the mean is from zero.
@@ -207,11 +257,15 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                d[j][e] = LAYOUT == ROWS_WHOLE ? d[j][e] - masked(m, own[j][0]) : masked(d[j][e] - m, own[j][e]);
-                two[0] += d[j][e];
-                two[1] = fmaf(d[j][e], d[j][e], two[1]);
+            for (int e = 0; e < E; e += 2) {
+                float2 v = add2(pair(&d[j][e]), both(LAYOUT == ROWS_WHOLE ? masked(-m, own[j][0]) : -m));
+                if (LAYOUT != ROWS_WHOLE) v = make_float2(masked(v.x, own[j][e]), masked(v.y, own[j][e + 1]));
+                part[1][e / 2 % 2] = add2(part[1][e / 2 % 2], v);
+                part[2][e / 2 % 2] = fma2(v, v, part[2][e / 2 % 2]);
+                unpair(v, &d[j][e]);
             }
+        two[0] = sum4(part[1]);
+        two[1] = sum4(part[2]);
         group_sum<L, 2>(two, s_two, turn_two);
         const float off = two[0] * p.inv_cols;
         const float var = fmaf(-off, off, two[1] * p.inv_cols);
@@ -220,7 +274,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) d[j][e] = fmaf(fmaf(d[j][e], s, shifted), w[j][e], b[j][e]);
+            for (int e = 0; e < E; e += 2) unpair(fma2(fma2(pair(&d[j][e]), both(s), both(shifted)), pair(&w[j][e]), pair(&b[j][e])), &d[j][e]);
         if (p.relu) {
 #pragma unroll
             for (int j = 0; j < CH; j++)
@@ -228,12 +282,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
                 for (int e = 0; e < E; e++) d[j][e] = relu_of(d[j][e]);
         }
         if (p.mask.on) {
-            uint32_t word[CH][E];
-            draw_words<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, word);
-#pragma unroll
-            for (int j = 0; j < CH; j++)
-#pragma unroll
-                for (int e = 0; e < E; e++) d[j][e] = word[j][e] >= p.mask.threshold ? d[j][e] : 0.f;
+            drop<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, d);
         }
         if (live) {
             if (p.stats != nullptr && at.t == 0) *stats = make_float2(m + off, s);
@@ -243,6 +292,22 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         stats += at.groups;
         block += p.part.words;
     }
+}
+
+// Bit j * E + e: whether z <= 0 in column c0 + j * stride + e.  Out of line, so that it takes no registers where it is not called.
+template <typename T>
+__device__ __noinline__ uint32_t closed_in_64_bits(const T *row, const float *weight, const float *bias, float2 stats, int c0, int stride, int chunks, int cols)
+{
+    constexpr int E = Elem<T>::E;
+    uint32_t bits = 0;
+    for (int j = 0; j < chunks; j++)
+        for (int e = 0; e < E; e++) {
+            const int c = c0 + j * stride + e;
+            if (c < 0 || c >= cols) continue;
+            const double h = ((double)Elem<T>::get(row[c]) - (double)stats.x) * (double)stats.y;
+            if (h * (weight != nullptr ? (double)weight[c] : 1.0) + (bias != nullptr ? (double)bias[c] : 0.0) <= 0.0) bits |= 1u << (j * E + e);
+        }
+    return bits;
 }
 
 template <typename T, int L, int CH, int LAYOUT>
@@ -258,15 +323,16 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
         __syncthreads();
     }
     const int cols = p.cols;
-    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols, p.mask);
+    const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols);
 
     extern __shared__ uint4 s_ring[];
-    RowRing<T, 2, CH, NORM_STAGES> ring(s_ring);
+    constexpr int STAGES = norm_backward_stages(L, E);
+    RowRing<T, 2, CH, STAGES> ring(s_ring);
     const T *const x_first = static_cast<const T *>(p.x), *const dy_first = static_cast<const T *>(p.dy);
     const T *x = x_first + at.group * p.ldx + at.column(0), *dy = dy_first + at.group * p.lddy + at.column(0);
     if (VEC) {
 #pragma unroll
-        for (int k = 0; k < NORM_STAGES; k++) {
+        for (int k = 0; k < STAGES; k++) {
             ring.clear();
             if (k < at.turns) {
                 at.fetch(ring, 0, x, x_first, cols);
@@ -279,23 +345,30 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
         }
     }
 
-    float w[CH][E], b[CH][E], sum_w[CH][E], sum_b[CH][E];
+    uint4 *s_columns = s_ring + STAGES * 2 * CH * blockDim.x;
+    NormColumns<L == 0, CH, E> w(s_columns), b(s_columns + CH * (E / 4) * blockDim.x);
+    float sum_w[CH][E], sum_b[CH][E];
     uint32_t own[CH][E];
     float uncertain = 0.f;
 #pragma unroll
-    for (int j = 0; j < CH; j++)
+    for (int j = 0; j < CH; j++) {
+        float wj[E], bj[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int c = at.column(j) + e;
             const bool in = c >= 0 && c < cols;
-            w[j][e] = in && p.weight != nullptr ? p.weight[c] : 1.f;
-            b[j][e] = !in ? INFINITY : p.bias != nullptr ? p.bias[c] : 0.f;       // a column that is not there is never near zero
+            wj[e] = in && p.weight != nullptr ? p.weight[c] : 1.f;
+            bj[e] = !in ? INFINITY : p.bias != nullptr ? p.bias[c] : 0.f;       // a column that is not there is never near zero
             // z = h w + b is off by less than 2^-22 |b| where the two terms cancel: its sign is not certain below that
-            if (in) uncertain = fmaxf(uncertain, fabsf(b[j][e]) * 4.76837158e-7f);
+            if (in) uncertain = fmaxf(uncertain, fabsf(bj[e]) * 4.76837158e-7f);
             sum_w[j][e] = sum_b[j][e] = 0.f;
             own[j][e] = at.mine(j, e);
         }
+        w.put(j, wj);
+        b.put(j, bj);
+    }
     const float scale = p.mask.on ? p.mask.scale : 1.f;       // of all gradients: once per row and at the end
+    const float dx_scale = cols > 1 ? scale : 0.f;            // (a row of one column is its own mean: its gradient is zero, not a rounding)
     const int64_t offset = mask_offset(p.mask);
     const int64_t number = p.mask.first + at.group * cols - at.shift;
     const int skip = (int)(number & 3);
@@ -307,18 +380,18 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
     for (int k = 0; k < at.warp_turns; k++) {
         const bool live = k < at.turns;
         float h[CH][E], g[CH][E];
-        float two[2] = {0.f, 0.f};
+        float2 part[2][2] = {};
         const float2 stats = next_stats;
         stats_at += at.groups;
         if (k + 1 < at.turns) next_stats = *stats_at;
         if (VEC) {
-            wait_copies<NORM_STAGES - 1>();
+            wait_copies<STAGES - 1>();
 #pragma unroll
             for (int j = 0; j < CH; j++) {
                 ring.get(0, j, h[j]);
                 ring.get(1, j, g[j]);
             }
-            if (k + NORM_STAGES < at.turns) {
+            if (k + STAGES < at.turns) {
                 at.fetch(ring, 0, x, x_first, cols);
                 at.fetch(ring, 1, dy, dy_first, cols);
             }
@@ -334,70 +407,74 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
 #pragma unroll
         for (int j = 0; j < CH; j++)
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                // what else a slot holds does not count
-                if (LAYOUT == ROWS_WHOLE) {
-                    h[j][e] = (h[j][e] - masked(stats.x, own[j][0])) * stats.y;
-                } else {
-                    h[j][e] = masked((h[j][e] - stats.x) * stats.y, own[j][e]);
-                    g[j][e] = masked(g[j][e], own[j][e]);
+            for (int e = 0; e < E; e += 2) {
+                unpair(mul2(add2(pair(&h[j][e]), both(LAYOUT == ROWS_WHOLE ? masked(-stats.x, own[j][0]) : -stats.x)), both(stats.y)), &h[j][e]);
+                if (LAYOUT != ROWS_WHOLE) {
+                    // what else a slot holds does not count
+#pragma unroll
+                    for (int i = e; i < e + 2; i++) {
+                        h[j][i] = masked(h[j][i], own[j][i]);
+                        if (LAYOUT == ROWS_EDGES && j == 0) g[j][i] = masked(g[j][i], own[j][i]);      // what is behind a row is 0
+                    }
                 }
             }
         if (p.relu) {
             bool near = false;
 #pragma unroll
-            for (int j = 0; j < CH; j++)
+            for (int j = 0; j < CH; j++) {
+                float wj[E], bj[E];
+                w.get(j, wj);
+                b.get(j, bj);
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const float z = fmaf(h[j][e], w[j][e], b[j][e]);
-                    near = near || fabsf(z) < uncertain;
-                    g[j][e] = relu_passes(z) ? g[j][e] : 0.f;
+                for (int e = 0; e < E; e += 2) {
+                    const float2 z = fma2(pair(&h[j][e]), pair(&wj[e]), pair(&bj[e]));
+                    near = near || fabsf(z.x) < uncertain || fabsf(z.y) < uncertain;
+                    g[j][e] = relu_passes(z.x) ? g[j][e] : 0.f;
+                    g[j][e + 1] = relu_passes(z.y) ? g[j][e + 1] : 0.f;
                 }
+            }
             if (near && live) {
                 // One element in millions: in 64 bits, so that a gradient passes where the formula lets it pass.
-                const int ahead = VEC ? NORM_STAGES : 0;
+                const int ahead = VEC ? STAGES : 0;
+                const uint32_t closed = closed_in_64_bits(x - ahead * p.x_step - at.column(0), p.weight, p.bias, stats, at.column(0), at.lanes * E, CH, cols);
 #pragma unroll
                 for (int j = 0; j < CH; j++) {
-                    load_chunk<T, false>(x - ahead * p.x_step - at.column(0), at.column(j), cols, h[j]);
                     load_chunk<T, false>(dy - ahead * p.dy_step - at.column(0), at.column(j), cols, g[j]);
 #pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const double d = (double)h[j][e] - (double)stats.x;
-                        if (d * (double)stats.y * (double)w[j][e] + (double)b[j][e] <= 0.0) g[j][e] = 0.f;
-                        h[j][e] = at.ok >> (j * E + e) & 1u ? (h[j][e] - stats.x) * stats.y : 0.f;
-                    }
+                    for (int e = 0; e < E; e++) g[j][e] = closed >> (j * E + e) & 1u ? 0.f : g[j][e];
                 }
             }
         }
         x += p.x_step;
         dy += p.dy_step;
         if (p.mask.on) {
-            uint32_t word[CH][E];
-            draw_words<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, word);
-#pragma unroll
-            for (int j = 0; j < CH; j++)
-#pragma unroll
-                for (int e = 0; e < E; e++) g[j][e] = word[j][e] >= p.mask.threshold ? g[j][e] : 0.f;
+            drop<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, g);
         }
         if (live) {
 #pragma unroll
-            for (int j = 0; j < CH; j++)
+            for (int j = 0; j < CH; j++) {
+                float wj[E];
+                w.get(j, wj);
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    sum_w[j][e] = fmaf(g[j][e], h[j][e], sum_w[j][e]);
-                    sum_b[j][e] += g[j][e];
-                    g[j][e] *= w[j][e];
-                    two[0] += g[j][e];
-                    two[1] = fmaf(g[j][e], h[j][e], two[1]);
+                for (int e = 0; e < E; e += 2) {
+                    float2 v = pair(&g[j][e]);
+                    unpair(fma2(v, pair(&h[j][e]), pair(&sum_w[j][e])), &sum_w[j][e]);
+                    unpair(add2(v, pair(&sum_b[j][e])), &sum_b[j][e]);
+                    v = mul2(v, pair(&wj[e]));
+                    part[0][e / 2 % 2] = add2(part[0][e / 2 % 2], v);
+                    part[1][e / 2 % 2] = fma2(v, pair(&h[j][e]), part[1][e / 2 % 2]);
+                    unpair(v, &g[j][e]);
                 }
+            }
         }
+        float two[2] = {sum4(part[0]), sum4(part[1])};
         group_sum<L, 2>(two, s_two, turn);
         if (live) {
-            const float s = stats.y * scale, m1 = two[0] * p.inv_cols * s, m2 = two[1] * p.inv_cols * s;
+            const float s = stats.y * dx_scale, m1 = two[0] * p.inv_cols * s, m2 = two[1] * p.inv_cols * s;
 #pragma unroll
             for (int j = 0; j < CH; j++)
 #pragma unroll
-                for (int e = 0; e < E; e++) g[j][e] = fmaf(-h[j][e], m2, fmaf(g[j][e], s, -m1));
+                for (int e = 0; e < E; e += 2) unpair(fma2(pair(&h[j][e]), both(-m2), fma2(pair(&g[j][e]), both(s), both(-m1))), &g[j][e]);
             at.template store<VEC>(dx, cols, g);
         }
         dx += p.dx_step;

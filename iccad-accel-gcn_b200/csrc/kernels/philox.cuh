@@ -44,17 +44,17 @@ __device__ __forceinline__ void philox4x32(const DropoutMask &m, int64_t offset,
     }
 }
 
-// Words of CH chunks of E elements; chunk j begins with word `skip` (0 to 3, alike for all) of block `block` + j * stride.
-// Element e is kept if its word is at least m.threshold.  (Where the chunks do not begin with a block, a word stands for
-// the answer: 0, or all ones.)
+// Words of CH chunks of E elements; chunk j begins with word `skip` (0 to 3, alike for all) of block `block[j]`.  Element e
+// is kept if its word is at least m.threshold.  (Where the chunks do not begin with a block, a word stands for the answer:
+// 0, or all ones.)
 template <int CH, int E>
-__device__ __forceinline__ void draw_words(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, uint32_t (&word)[CH][E])
+__device__ __forceinline__ void draw_words(const DropoutMask &m, int64_t offset, const int64_t (&block)[CH], int skip, uint32_t (&word)[CH][E])
 {
     constexpr int B = E / 4;
     int64_t blocks[CH * B];
     uint32_t w[CH * B][4];
 #pragma unroll
-    for (int n = 0; n < CH * B; n++) blocks[n] = block + (n / B) * stride + n % B;
+    for (int n = 0; n < CH * B; n++) blocks[n] = block[n / B] + n % B;
     philox4x32<CH * B>(m, offset, blocks, w);
 #pragma unroll
     for (int j = 0; j < CH; j++)
@@ -64,7 +64,7 @@ __device__ __forceinline__ void draw_words(const DropoutMask &m, int64_t offset,
         int64_t more[CH];
         uint32_t v[CH][4];
 #pragma unroll
-        for (int j = 0; j < CH; j++) more[j] = block + j * stride + B;
+        for (int j = 0; j < CH; j++) more[j] = block[j] + B;
         philox4x32<CH>(m, offset, more, v);
 #pragma unroll
         for (int j = 0; j < CH; j++) {

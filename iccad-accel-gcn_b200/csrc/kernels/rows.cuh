@@ -6,6 +6,11 @@
 
 namespace agcn {
 
+// How the rows of all tensors of a call sit: alike with respect to 16-byte boundaries, every row beginning and ending on
+// one (WHOLE); alike, with chunks at the rows' ends that are not the row's alone (EDGES); or not alike (LOOSE: read
+// element by element).
+enum RowLayout { ROWS_WHOLE, ROWS_EDGES, ROWS_LOOSE };
+
 // E elements of type T are 16 bytes.  All arithmetic is in fp32; the one rounding to T is that of the result.
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -66,6 +71,33 @@ template <> struct Elem<__half> {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
+
+// Two fp32 operations in one instruction (both rounded as the single ones are): these kernels are bound by the instructions
+// that can be issued long before the arithmetic units are full.
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 pair(const float *v) { return make_float2(v[0], v[1]); }
+__device__ __forceinline__ void unpair(float2 p, float *v) { v[0] = p.x; v[1] = p.y; }
 
 // Columns c0 .. c0 + E - 1 of a row, as far as they are in [0, cols); zeros elsewhere.  VEC: a whole chunk is one access
 // (column c0 then sits on a 16-byte boundary); the chunks at the ends of a row go element by element, so that nothing
@@ -167,7 +199,7 @@ __device__ __forceinline__ bool relu_passes(float v) { return !(v <= 0.f); }
 // Sums of K values over a group of L lanes of a warp, or (L = 0) over the thread block; every thread gets them, added
 // in one order.  All lanes of the warp (threads of the block) call.  s_sums: zero where there is no warp; `turn` says which half is
 // free: the other one may still be read by warps that are behind.
-constexpr int ROW_WARPS = 20;              // most warps of a thread block that has one row, a multiple of 4
+constexpr int ROW_WARPS = 16;              // most warps of a thread block that has one row
 template <int K> struct GroupSums { alignas(16) float v[2][K][ROW_WARPS]; };
 template <int K>
 __device__ __forceinline__ void clear_sums(GroupSums<K> &s)
@@ -177,25 +209,31 @@ __device__ __forceinline__ void clear_sums(GroupSums<K> &s)
 template <int L, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], GroupSums<K> &s_sums, int &turn)
 {
-    constexpr int W = L > 0 ? L : 32;
+    static_assert(K == 1 || K == 2, "");
+    if (L > 0) {
 #pragma unroll
-    for (int d = W / 2; d > 0; d >>= 1) {
+        for (int d = L / 2; d > 0; d >>= 1) {
 #pragma unroll
-        for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], d);
-    }
-    if (L == 0) {
-        if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-            for (int k = 0; k < K; k++) s_sums.v[turn][k][threadIdx.x >> 5] = v[k];
+            for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], d);
         }
+    } else {
+        // Half of the lanes add up one value and half the other: one exchange more than for one value, not five.
+        const int lane = threadIdx.x & 31;
+        float s = v[0];
+        if (K == 2) s = (lane & 16 ? v[K - 1] : v[0]) + __shfl_xor_sync(0xffffffffu, lane & 16 ? v[0] : v[K - 1], 16);
+        else s += __shfl_xor_sync(0xffffffffu, s, 16);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if ((lane & 15) == 0) s_sums.v[turn][K == 2 ? lane >> 4 : 0][threadIdx.x >> 5] = s;
         __syncthreads();
+        s = s_sums.v[turn][K == 2 ? lane >> 4 : 0][lane & 15];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const float4 *q = reinterpret_cast<const float4 *>(s_sums.v[turn][k]);
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < ROW_WARPS / 4; i++) s += (q[i].x + q[i].y) + (q[i].z + q[i].w);
-            v[k] = s;
+        for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        v[0] = s;
+        if (K == 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+            v[0] = lane & 16 ? other : s;
+            v[K - 1] = lane & 16 ? s : other;
         }
         turn ^= 1;
     }

@@ -11,14 +11,14 @@ struct NormForwardLaunch {
     template <typename T, int L, int CH, int LAYOUT> int operator()() const
     {
         int64_t resident = 0;
-        const int rc = norm_resident<layer_norm_kernel<T, L, CH, LAYOUT>>(f.threads, norm_smem(f, 1), &resident);
+        const int rc = norm_resident<layer_norm_kernel<T, L, CH, LAYOUT>>(f.threads, norm_smem(f, 1, Elem<T>::E), &resident);
         if (rc != AGCN_OK) return rc;
         const int64_t grid = norm_grid(f, p.rows, resident);
         int64_t groups = 0;
         p.part = norm_rows(f, grid, p.rows, p.cols, &groups);
         p.x_step = groups * p.ldx;
         p.y_step = groups * p.ldy;
-        layer_norm_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 1), s>>>(p);
+        layer_norm_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 1, Elem<T>::E), s>>>(p);
         AGCN_LAUNCH_CHECK("layer_norm_kernel");
         return AGCN_OK;
     }
@@ -49,6 +49,6 @@ extern "C" int agcn_layer_norm(const void *d_x, int64_t ldx, const float *d_weig
     a.stats = reinterpret_cast<float2 *>(d_stats);
     a.cols = (int)cols; a.relu = activation == AGCN_ACT_RELU;
     a.eps = (float)eps; a.inv_cols = 1.f / (float)cols;
-    const NormForm f = norm_form(t, 2, cols, dtype, a.mask.on, NORM_FORWARD_ELEMS);
+    const NormForm f = norm_form(t, 2, cols, dtype, NORM_FORWARD_ELEMS);
     return norm_dispatch(f, dtype, NormForwardLaunch{a, f, static_cast<cudaStream_t>(stream)});
 }

@@ -7,8 +7,9 @@ namespace agcn {
 
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
-constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
-constexpr int NORM_MAX_SMEM = NORM_STAGES * 2 * NORM_ELEMS * 4 * NORM_MAX_THREADS;
+constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8, NORM_EDGE_ELEMS = 8;
+constexpr int NORM_MAX_SMEM = 200 * 1024;
+static_assert(NORM_MAX_THREADS * NORM_ELEMS * (norm_backward_stages(0, 4) * 2 * 4 + 8) <= NORM_MAX_SMEM, "8192 columns in 32 bits");
 
 struct NormForm {
     int layout;                             // RowLayout
@@ -19,14 +20,17 @@ struct NormForm {
 };
 
 // `per_lane`: elements of a row per lane of a group within a warp that are aimed at
-inline NormForm norm_form(const Rows *t, int n, int64_t cols, int dtype, bool mask, int per_lane)
+inline NormForm norm_form(const Rows *t, int n, int64_t cols, int dtype, int per_lane)
 {
     const int e = 16 / dtype_bytes(dtype), most_chunks = NORM_ELEMS / e;
     NormForm f = {};
     int shift = 0;
-    f.layout = !rows_sit_alike(t, n, dtype, &shift) ? ROWS_LOOSE : shift != 0 || cols % e != 0 ? ROWS_EDGES : ROWS_WHOLE;
-    if (f.layout == ROWS_LOOSE) shift = mask ? 3 : 0;
+    f.layout = rows_layout(t, n, cols, dtype, &shift);
+    // the one thread block that has a row has no room for a chunk more
+    if (cols + shift > NORM_MAX_COLS) f.layout = ROWS_LOOSE;
+    if (f.layout == ROWS_LOOSE) shift = 0;
     const int chunks = (int)ceil_div(cols + shift, e);
+    if (f.layout == ROWS_EDGES && per_lane > NORM_EDGE_ELEMS) per_lane = NORM_EDGE_ELEMS;
     f.lanes = 2;
     while (f.lanes < 32 && f.lanes * per_lane / e < chunks) f.lanes *= 2;
     f.threads = NORM_THREADS;
@@ -82,8 +86,13 @@ template <typename F> int norm_dispatch(const NormForm &f, int dtype, F &&launch
     return dtype == AGCN_BF16 ? norm_dispatch_layout<__nv_bfloat16>(f, launch) : norm_dispatch_layout<__half>(f, launch);
 }
 
-// Dynamic shared memory: the ring of `tensors` tensors, and at the end the groups' column sums
-inline int norm_smem(const NormForm &f, int tensors) { return NORM_STAGES * tensors * f.chunks * f.threads * 16; }
+// Dynamic shared memory: the ring of `tensors` tensors (at the end the groups' column sums) and, where a thread block has one
+// row, weight and bias of the backward pass
+inline int norm_smem(const NormForm &f, int tensors, int elems)
+{
+    const int stages = tensors == 2 ? norm_backward_stages(f.lanes, elems) : NORM_STAGES;
+    return f.threads * f.chunks * (stages * tensors * 16 + (f.lanes == 0 && tensors == 2 ? 8 * elems : 0));
+}
 
 inline NormRows norm_rows(const NormForm &f, int64_t grid, int64_t rows, int64_t cols, int64_t *groups)
 {

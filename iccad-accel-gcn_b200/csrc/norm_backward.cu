@@ -21,7 +21,7 @@ struct NormBackwardLaunch {
     template <typename T, int L, int CH, int LAYOUT> int operator()() const
     {
         int64_t resident = 0;
-        const int rc = norm_resident<layer_norm_backward_kernel<T, L, CH, LAYOUT>>(f.threads, norm_smem(f, 2), &resident);
+        const int rc = norm_resident<layer_norm_backward_kernel<T, L, CH, LAYOUT>>(f.threads, norm_smem(f, 2, Elem<T>::E), &resident);
         if (rc != AGCN_OK) return rc;
         float *dweight = p.dweight, *dbias = p.dbias;
         const int64_t grid = norm_grid(f, p.rows, resident < most_parts ? resident : most_parts);
@@ -37,7 +37,7 @@ struct NormBackwardLaunch {
         p.dy_step = groups * p.lddy;
         p.x_step = groups * p.ldx;
         p.dx_step = groups * p.lddx;
-        layer_norm_backward_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 2), s>>>(p);
+        layer_norm_backward_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 2, Elem<T>::E), s>>>(p);
         AGCN_LAUNCH_CHECK("layer_norm_backward_kernel");
         if (sums) {
             norm_columns_kernel<<<dim3((unsigned)ceil_div(p.cols, 32), 2), 256, 0, s>>>(work, p.part_stride, (int)grid, dweight, dbias, p.cols);
@@ -98,6 +98,6 @@ extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const vo
     a.dweight = d_dweight; a.dbias = d_dbias;
     a.cols = (int)cols; a.relu = activation == AGCN_ACT_RELU;
     a.inv_cols = 1.f / (float)cols;
-    const NormForm f = norm_form(t, 3, cols, dtype, a.mask.on, NORM_BACKWARD_ELEMS);
+    const NormForm f = norm_form(t, 3, cols, dtype, NORM_BACKWARD_ELEMS);
     return norm_dispatch(f, dtype, NormBackwardLaunch{a, f, static_cast<float *>(d_work), parts, s});
 }

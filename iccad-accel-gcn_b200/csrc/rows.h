@@ -2,6 +2,7 @@
 #pragma once
 #include "host_common.h"
 #include "kernels/philox.cuh"
+#include "kernels/rows.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,15 +56,16 @@ inline int make_mask(const char *who, DropoutMask *m, double p, int64_t seed, in
     return AGCN_OK;
 }
 
-// Whether all tensors' rows sit alike with respect to 16-byte boundaries; *most: elements that a row may begin behind one.
-inline bool rows_sit_alike(const Rows *t, int n, int dtype, int *most)
+// How the rows of all tensors sit; *most: elements that a row may begin behind a 16-byte boundary.
+inline int rows_layout(const Rows *t, int n, int64_t cols, int dtype, int *most)
 {
     const int size = dtype_bytes(dtype), e = 16 / size;
     const auto at = [&](const Rows &r) { return (int)(reinterpret_cast<uintptr_t>(r.ptr) / size % e); };
+    *most = 0;
     for (int k = 1; k < n; k++)
-        if (at(t[k]) != at(t[0]) || t[k].ld % e != t[0].ld % e) return false;
+        if (at(t[k]) != at(t[0]) || t[k].ld % e != t[0].ld % e) return ROWS_LOOSE;
     *most = t[0].ld % e == 0 ? at(t[0]) : e - 1;
-    return true;
+    return *most != 0 || cols % e != 0 ? ROWS_EDGES : ROWS_WHOLE;
 }
 
 // Streaming multiprocessors of the current device, looked up once
