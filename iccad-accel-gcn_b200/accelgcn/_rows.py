@@ -1,58 +1,68 @@
-"""What the row-wise operators (norm, dropout) ask of their tensors before the library sees a pointer."""
+"""What the row-wise operators (norm, dropout) ask of their tensors before the library sees a pointer.
+
+A call on a graph of a few thousand nodes takes 3 us on the GPU; every attribute of a tensor that Python asks for is 50 to
+100 ns, so each is asked for once and compared in the cheapest way."""
 from __future__ import annotations
 
 import contextlib
-from operator import index
 
 import torch
 
 from . import _lib
 
+F32 = torch.float32
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # AGCN_F32, AGCN_BF16, AGCN_F16
 
 
-def features(name, t, like=None):
-    """Checks [rows, cols] features with unit column stride (of the shape, type and device of `like`); returns the row stride."""
-    if not t.is_cuda or t.dtype not in DTYPES:
+def features(name, t):
+    """(rows, cols, row stride, type code, type, device index) of [rows, cols] features with unit column stride."""
+    dtype, dev = t.dtype, t.get_device()
+    code = DTYPES.get(dtype)
+    if dev < 0 or code is None:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must be [rows, cols]")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} must have the shape, type and device of the other features")
-    rows, cols = t.shape
+    rows, cols = shape
     ld, inner = t.stride()
-    if cols > 1 and inner != 1:
-        raise ValueError(f"{name} must have unit column stride")
     if rows <= 1:
-        return cols
-    if ld < cols:
-        raise ValueError(f"rows of {name} overlap (stride {ld}): copy it first")
+        ld = cols
+    if (inner != 1 and cols > 1) or ld < cols:
+        raise ValueError(f"{name} must have unit column stride and rows that do not overlap (strides {ld}, {inner}): copy it first")
+    return rows, cols, ld, code, dtype, dev
+
+
+def more_features(name, t, rows, cols, dtype, dev):
+    """The row stride of features that must be like others."""
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must have the type and device of the other features")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise ValueError(f"{name} must be [{rows}, {cols}] like the other features")
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = cols
+    if (inner != 1 and cols > 1) or ld < cols:
+        raise ValueError(f"{name} must have unit column stride and rows that do not overlap (strides {ld}, {inner}): copy it first")
     return ld
 
 
-def array(name, t, dtype, shape, like):
-    """Checks a contiguous array on the features' device; returns its address (None where there is none)."""
+def array(name, t, shape, dev):
+    """Address of a contiguous float32 array on the features' device (None where there is none)."""
     if t is None:
         return None
-    if not t.is_cuda or t.dtype != dtype or t.device != like.device:
-        raise TypeError(f"{name} must be a {dtype} tensor on the features' device")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not F32 or t.get_device() != dev:
+        raise TypeError(f"{name} must be a float32 tensor on the features' device")
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {list(shape)}")
     return t.data_ptr()
 
 
-def step_address(step, like):
+def step_address(step, dev):
     """Address of the device counter that is added to a mask's offset."""
-    if step is None:
-        return None
-    if not step.is_cuda or step.dtype != torch.int64 or step.device != like.device or step.numel() != 1:
+    if step.dtype is not torch.int64 or step.get_device() != dev or step.numel() != 1:
         raise TypeError("step must be one int64 on the features' device")
     return step.data_ptr()
-
-
-def mask_numbers(p, seed, offset, row0):
-    """As the library takes them: what is no integer must not become a double on the way."""
-    return float(p), index(seed), index(offset), index(row0)
 
 
 _NO_CONTEXT = contextlib.nullcontext()
@@ -63,5 +73,30 @@ def allocating_on(stream):
     return _NO_CONTEXT if stream is None else torch.cuda.stream(stream)
 
 
-def stream_of(stream, dev):
-    return stream.cuda_stream if stream is not None else _lib.raw_stream(dev)
+def empty(rows, cols, dtype, dev, stream):
+    with allocating_on(stream):
+        return torch.empty((rows, cols), dtype=dtype, device=f"cuda:{dev}")
+
+
+_address = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_call = None
+
+
+def run(function, dev, stream, *args):
+    """The library's `function` on device `dev`, its last argument the stream (None: the current one)."""
+    global _call
+    if _call is None:
+        _lib.load()
+        _call = _lib.call()
+    address = _address.get(function)
+    if address is None:
+        address = _address[function] = _lib.address(function)
+    s = _raw_stream(dev) if stream is None else stream.cuda_stream
+    if torch._C._cuda_getDevice() == dev:
+        rc = _call(address, *args, s)
+    else:
+        with torch.cuda.device(dev):
+            rc = _call(address, *args, s)
+    if rc != 0:
+        _lib.check(rc)

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from operator import index
 
 import torch
 
@@ -26,21 +27,16 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, relu: bool = False,
     [rows, 2], receives mean and 1 / sqrt(variance + eps) of the rows: what the backward pass needs.  row0: where this
     rank's rows begin in the whole.  step: an int64 on the device that is added to `offset` when the kernel runs (a captured
     graph counts it up to have new masks).  out may be x.  Asynchronous on the current stream (or `stream`)."""
-    ldx = _rows.features("x", x)
-    with _rows.allocating_on(stream):
-        y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ldy = _rows.features("out", y, x)
-    rows, cols = x.shape
-    dev = _lib.device_index(x.device)
-    p, seed, offset, row0 = _rows.mask_numbers(p, seed, offset, row0)
-    args = (x.data_ptr(), ldx, _rows.array("weight", weight, torch.float32, (cols,), x), _rows.array("bias", bias, torch.float32, (cols,), x),
-            float(eps), y.data_ptr(), ldy, _rows.array("stats", stats, torch.float32, (rows, 2), x), rows, cols, _rows.DTYPES[x.dtype],
-            1 if relu else 0, p, seed, offset, _rows.step_address(step, x), row0, _rows.stream_of(stream, dev))
-    with _lib.on_device(dev):
-        rc = _lib.call()(_lib.address("agcn_layer_norm"), *args)
-    if rc != 0:
-        _lib.check(rc)
-    return y
+    rows, cols, ldx, code, dtype, dev = _rows.features("x", x)
+    if out is None:
+        out, ldy = _rows.empty(rows, cols, dtype, dev, stream), cols
+    else:
+        ldy = _rows.more_features("out", out, rows, cols, dtype, dev)
+    vector = (cols,)
+    _rows.run("agcn_layer_norm", dev, stream, x.data_ptr(), ldx, _rows.array("weight", weight, vector, dev), _rows.array("bias", bias, vector, dev),
+              float(eps), out.data_ptr(), ldy, None if stats is None else _rows.array("stats", stats, (rows, 2), dev), rows, cols, code,
+              1 if relu else 0, float(p), index(seed), index(offset), None if step is None else _rows.step_address(step, dev), index(row0))
+    return out
 
 
 @functools.lru_cache(maxsize=4096)
@@ -56,31 +52,31 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None, relu: bool = False
     """Gradients of `layer_norm`: (dx, dweight, dbias) from dy, and the x, stats, weight, bias and mask numbers of the forward
     pass.  dweight and dbias are float32 [cols], overwritten, the same bits from run to run; None where there was no weight (bias)
     and no array is given for it.  dx may be dy or x.  Asynchronous on the current stream (or `stream`)."""
-    lddy = _rows.features("dy", dy)
-    ldx = _rows.features("x", x, dy)
-    rows, cols = x.shape
-    dev, dtype = _lib.device_index(x.device), _rows.DTYPES[x.dtype]
+    rows, cols, ldx, code, dtype, dev = _rows.features("x", x)
+    lddy = _rows.more_features("dy", dy, rows, cols, dtype, dev)
     if stats is None:
         raise TypeError("layer_norm_backward needs the stats of the forward pass")
-    with _rows.allocating_on(stream):
-        if dx is None:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if dweight is None and weight is not None:
-            dweight = torch.empty(cols, dtype=torch.float32, device=x.device)
-        if dbias is None and bias is not None:
-            dbias = torch.empty(cols, dtype=torch.float32, device=x.device)
-        # of this call alone: calls on other streams, and captured graphs, have their own
-        n = _work_floats(dev, rows, cols, dtype) if dweight is not None or dbias is not None else 0
-        work = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-    lddx = _rows.features("dx", dx, x)
-    p, seed, offset, row0 = _rows.mask_numbers(p, seed, offset, row0)
-    args = (dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.array("stats", stats, torch.float32, (rows, 2), x),
-            _rows.array("weight", weight, torch.float32, (cols,), x), _rows.array("bias", bias, torch.float32, (cols,), x), dx.data_ptr(), lddx,
-            _rows.array("dweight", dweight, torch.float32, (cols,), x), _rows.array("dbias", dbias, torch.float32, (cols,), x),
-            work.data_ptr() if n else None, 4 * n, rows, cols, dtype, 1 if relu else 0, p, seed, offset, _rows.step_address(step, x), row0,
-            _rows.stream_of(stream, dev))
-    with _lib.on_device(dev):
-        rc = _lib.call()(_lib.address("agcn_layer_norm_backward"), *args)
-    if rc != 0:
-        _lib.check(rc)
+    if dx is None:
+        dx, lddx = _rows.empty(rows, cols, dtype, dev, stream), cols
+    else:
+        lddx = _rows.more_features("dx", dx, rows, cols, dtype, dev)
+    if (dweight is None and weight is not None) or (dbias is None and bias is not None):
+        with _rows.allocating_on(stream):
+            if dweight is None and weight is not None:
+                dweight = torch.empty(cols, dtype=_rows.F32, device=x.device)
+            if dbias is None and bias is not None:
+                dbias = torch.empty(cols, dtype=_rows.F32, device=x.device)
+    work, n = None, 0
+    if dweight is not None or dbias is not None:
+        n = _work_floats(dev, rows, cols, code)
+        if n:
+            # of this call alone: calls on other streams, and captured graphs, have their own
+            with _rows.allocating_on(stream):
+                work = torch.empty(n, dtype=_rows.F32, device=x.device)
+    vector = (cols,)
+    _rows.run("agcn_layer_norm_backward", dev, stream, dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.array("stats", stats, (rows, 2), dev),
+              _rows.array("weight", weight, vector, dev), _rows.array("bias", bias, vector, dev), dx.data_ptr(), lddx,
+              _rows.array("dweight", dweight, vector, dev), _rows.array("dbias", dbias, vector, dev), None if work is None else work.data_ptr(), 4 * n,
+              rows, cols, code, 1 if relu else 0, float(p), index(seed), index(offset), None if step is None else _rows.step_address(step, dev),
+              index(row0))
     return dx, dweight, dbias

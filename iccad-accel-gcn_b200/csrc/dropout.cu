@@ -24,8 +24,7 @@ template <auto KERNEL> static int dropout_start(const DropoutParams &p, int64_t 
     if (rc != AGCN_OK) return rc;
     const int64_t needed = ceil_div(threads, DROPOUT_THREADS);
     resident = resident / 8 * 8;
-    KERNEL<<<(unsigned)(needed < resident ? needed : resident), DROPOUT_THREADS, 0, s>>>(p);
-    AGCN_LAUNCH_CHECK("dropout kernel");
+    AGCN_CUDA(launch_early(true, KERNEL, (unsigned)(needed < resident ? needed : resident), DROPOUT_THREADS, 0, s, p));
     return AGCN_OK;
 }
 

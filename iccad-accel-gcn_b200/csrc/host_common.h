@@ -45,13 +45,13 @@ void clear_error();
 // Kernel launch that, if `early`, may start while the launch before it on the stream still runs (the kernel waits
 // for that one itself before it uses what it makes).
 template <typename... Params, typename... Args>
-inline cudaError_t launch_early(bool early, void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args... args)
+inline cudaError_t launch_early(bool early, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, Args... args)
 {
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cfg.attrs = &attr; cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }

@@ -5,6 +5,7 @@
 // in 16.
 #pragma once
 #include "philox.cuh"
+#include "ptx.cuh"
 #include "rows.cuh"
 
 namespace agcn {
@@ -97,6 +98,7 @@ __global__ void __launch_bounds__(DROPOUT_THREADS)
 dropout_array_kernel(const __grid_constant__ DropoutParams p)
 {
     constexpr int E = Elem<T>::E, U = DROPOUT_CHUNKS;
+    wait_for_predecessor();
     const int64_t offset = mask_offset(p.mask), n = p.rows * p.cols;
     const int shift = (int)((reinterpret_cast<uintptr_t>(p.v) / sizeof(T)) & (E - 1));
     const int64_t step = (int64_t)gridDim.x * DROPOUT_THREADS * E;
@@ -132,6 +134,7 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
 {
     constexpr bool WHOLE = LAYOUT == ROWS_WHOLE;
     constexpr int E = Elem<T>::E, U = DROPOUT_ROW_CHUNKS[LAYOUT], STAGES = DROPOUT_STAGES, TENSORS = GATE ? 2 : 1;
+    wait_for_predecessor();
     const int64_t offset = mask_offset(p.mask);
     const int64_t thread = (int64_t)blockIdx.x * DROPOUT_THREADS + threadIdx.x;
     const int64_t group = thread / p.lanes, groups = (int64_t)gridDim.x * (DROPOUT_THREADS / p.lanes);

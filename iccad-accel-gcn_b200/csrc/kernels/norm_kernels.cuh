@@ -12,7 +12,10 @@
 // bytes at a time (rows of tensors that do not sit alike are read element by element).  The next rows are under way
 // in a ring in shared memory meanwhile (RowRing).
 #pragma once
+#include <cooperative_groups.h>
+
 #include "philox.cuh"
+#include "ptx.cuh"
 #include "rows.cuh"
 
 namespace agcn {
@@ -52,8 +55,9 @@ struct NormBackward {
     int64_t lddy, ldx, lddx, rows;
     const float *weight, *bias;
     const float2 *stats;
-    float *dweight, *dbias;                // [gridDim.x][cols] each, one row per thread block; null: not wanted
+    float *dweight, *dbias;                // [gridDim.x][cols] each, one row per thread block; [cols] where all are one cluster; null: not wanted
     int64_t part_stride;                   // floats between two thread blocks' rows
+    int cluster;                           // whether the thread blocks are one cluster
     int cols, relu;
     float inv_cols;
     DropoutMask mask;
@@ -189,6 +193,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
 
     extern __shared__ uint4 s_ring[];
     RowRing<T, 1, CH, NORM_STAGES> ring(s_ring);
+    wait_for_predecessor();
     const T *const first = static_cast<const T *>(p.x), *x = first + at.group * p.ldx + at.column(0);
     if (VEC) {
 #pragma unroll
@@ -328,6 +333,7 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
     extern __shared__ uint4 s_ring[];
     constexpr int STAGES = norm_backward_stages(L, E);
     RowRing<T, 2, CH, STAGES> ring(s_ring);
+    wait_for_predecessor();
     const T *const x_first = static_cast<const T *>(p.x), *const dy_first = static_cast<const T *>(p.dy);
     const T *x = x_first + at.group * p.ldx + at.column(0), *dy = dy_first + at.group * p.lddy + at.column(0);
     if (VEC) {
@@ -482,13 +488,13 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
     }
 
     if (VEC) wait_copies<0>();
-    // The groups' sums, then the thread blocks': always in the same order.
+    // The groups' sums, then the thread blocks': always in the same order.  The ring is empty by now and has room for them.
+    float *s_cols = reinterpret_cast<float *>(s_ring), *s_parts = s_cols + (L > 0 ? NORM_THREADS * CH * E : 0);
 #pragma unroll
     for (int pass = 0; pass < 2; pass++) {
         float *part = pass == 0 ? p.dweight : p.dbias;
         if (part == nullptr) continue;
-        part += (int64_t)blockIdx.x * p.part_stride;
-        float *s_cols = reinterpret_cast<float *>(s_ring);       // the ring is empty by now
+        part = p.cluster ? s_parts + pass * cols : part + (int64_t)blockIdx.x * p.part_stride;
         if (L > 0) __syncthreads();
         float *mine = L > 0 ? s_cols + (threadIdx.x / (L > 0 ? L : 1)) * cols : part;
 #pragma unroll
@@ -505,6 +511,19 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
             }
         }
     }
+    if (p.cluster) {
+        // few rows: the thread blocks read each other's sums, in place of a second kernel and a workspace
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < 2 * cols; c += gridDim.x * blockDim.x) {
+            float *out = c < cols ? p.dweight : p.dbias;
+            if (out == nullptr) continue;
+            float s = 0.f;
+            for (unsigned k = 0; k < gridDim.x; k++) s += *cluster.map_shared_rank(s_parts + c, k);
+            out[c < cols ? c : c - cols] = s;
+        }
+        cluster.sync();                        // nobody leaves while its sums are read
+    }
 }
 
 // Column sums of the thread blocks' rows: 32 columns per thread block, its 8 warps over the rows in turn.
@@ -515,6 +534,7 @@ norm_columns_kernel(const float *__restrict__ parts, int64_t part_stride, int n_
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float *out = blockIdx.y == 0 ? dweight : dbias;
     if (out == nullptr) return;
+    wait_for_predecessor();
     float s = 0.f;
     if (c < cols)
         for (int k = warp; k < n_parts; k += 8) s += parts[k * part_stride + (int64_t)blockIdx.y * cols + c];

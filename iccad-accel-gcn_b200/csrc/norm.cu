@@ -18,8 +18,7 @@ struct NormForwardLaunch {
         p.part = norm_rows(f, grid, p.rows, p.cols, &groups);
         p.x_step = groups * p.ldx;
         p.y_step = groups * p.ldy;
-        layer_norm_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 1, Elem<T>::E), s>>>(p);
-        AGCN_LAUNCH_CHECK("layer_norm_kernel");
+        AGCN_CUDA(launch_early(true, layer_norm_kernel<T, L, CH, LAYOUT>, (unsigned)grid, f.threads, norm_smem(f, 1, Elem<T>::E), s, p));
         return AGCN_OK;
     }
 };

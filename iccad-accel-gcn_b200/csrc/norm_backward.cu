@@ -3,13 +3,20 @@
 
 namespace agcn {
 
-// Thread blocks per SM whose sums the workspace holds: all that are resident, for the forms there are
+// Whether a call's thread blocks are one cluster
+static bool norm_one_cluster(int64_t rows, int64_t cols, int dtype)
+{
+    const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
+    return rows <= NORM_CLUSTER * NORM_CLUSTER_TURNS * f.rows_per_block;
+}
+
+// Thread blocks whose sums the workspace holds: all that are resident, for the forms there are
 static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int sms)
 {
-    const int64_t chunks = ceil_div(cols, 16 / dtype_bytes(dtype)), per_warp = 32 * NORM_ELEMS / (16 / dtype_bytes(dtype));
-    const int64_t threads = chunks <= per_warp ? NORM_THREADS : 32 * ceil_div(chunks, per_warp);
-    const int64_t most = sms * (2048 / threads);
-    return rows < most ? (rows > 0 ? rows : 1) : most;
+    if (norm_one_cluster(rows, cols, dtype)) return 0;
+    const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
+    const int64_t most = sms * (2048 / f.threads);
+    return rows < most ? rows : most;
 }
 
 struct NormBackwardLaunch {
@@ -20,14 +27,20 @@ struct NormBackwardLaunch {
     cudaStream_t s;
     template <typename T, int L, int CH, int LAYOUT> int operator()() const
     {
+        constexpr auto kernel = layer_norm_backward_kernel<T, L, CH, LAYOUT>;
+        const size_t smem = norm_smem(f, 2, Elem<T>::E);
         int64_t resident = 0;
-        const int rc = norm_resident<layer_norm_backward_kernel<T, L, CH, LAYOUT>>(f.threads, norm_smem(f, 2, Elem<T>::E), &resident);
+        const int rc = norm_resident<layer_norm_backward_kernel<T, L, CH, LAYOUT>>(f.threads, (int)smem, &resident);
         if (rc != AGCN_OK) return rc;
         float *dweight = p.dweight, *dbias = p.dbias;
-        const int64_t grid = norm_grid(f, p.rows, resident < most_parts ? resident : most_parts);
-        const bool sums = (dweight != nullptr || dbias != nullptr) && grid > 1;
-        AGCN_REQUIRE(!sums || grid <= most_parts, "agcn_layer_norm_backward: the workspace is too small");
-        if (sums) {
+        const bool wanted = dweight != nullptr || dbias != nullptr;
+        int64_t grid = norm_grid(f, p.rows, resident);
+        if (wanted && most_parts == 0) {
+            const int64_t needed = ceil_div(p.rows, f.rows_per_block);
+            for (grid = 1; grid < needed && grid < NORM_CLUSTER; grid *= 2) {}
+            p.cluster = 1;
+        } else if (wanted) {
+            grid = norm_grid(f, p.rows, resident < most_parts ? resident : most_parts);
             p.part_stride = 2 * p.cols;
             p.dweight = dweight != nullptr ? work : nullptr;
             p.dbias = dbias != nullptr ? work + p.cols : nullptr;
@@ -37,12 +50,18 @@ struct NormBackwardLaunch {
         p.dy_step = groups * p.lddy;
         p.x_step = groups * p.ldx;
         p.dx_step = groups * p.lddx;
-        layer_norm_backward_kernel<T, L, CH, LAYOUT><<<(unsigned)grid, f.threads, norm_smem(f, 2, Elem<T>::E), s>>>(p);
-        AGCN_LAUNCH_CHECK("layer_norm_backward_kernel");
-        if (sums) {
-            norm_columns_kernel<<<dim3((unsigned)ceil_div(p.cols, 32), 2), 256, 0, s>>>(work, p.part_stride, (int)grid, dweight, dbias, p.cols);
-            AGCN_LAUNCH_CHECK("norm_columns_kernel");
-        }
+        cudaLaunchAttribute attr[2] = {};
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)grid; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(f.threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+        cfg.attrs = attr; cfg.numAttrs = p.cluster ? 2 : 1;
+        AGCN_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+        if (wanted && !p.cluster)
+            AGCN_CUDA(launch_early(true, norm_columns_kernel, dim3((unsigned)ceil_div(p.cols, 32), 2), 256, 0, s, work, p.part_stride, (int)grid, dweight,
+                                   dbias, p.cols));
         return AGCN_OK;
     }
 };
@@ -90,7 +109,7 @@ extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const vo
     int dev = 0, sms = 0;
     if ((rc = current_sm_count(&dev, &sms)) != AGCN_OK) return rc;
     const int64_t parts = norm_parts(rows, cols, dtype, sms);
-    AGCN_REQUIRE((d_dweight == nullptr && d_dbias == nullptr) || (d_work != nullptr && work_bytes >= parts * 2 * cols * (int64_t)sizeof(float)),
+    AGCN_REQUIRE((d_dweight == nullptr && d_dbias == nullptr) || parts == 0 || (d_work != nullptr && work_bytes >= parts * 2 * cols * (int64_t)sizeof(float)),
                  "%s: workspace of %lld bytes, %lld are needed", who, (long long)work_bytes, (long long)(parts * 2 * cols * (int64_t)sizeof(float)));
     a.dy = d_dy; a.lddy = lddy; a.x = d_x; a.ldx = ldx; a.dx = d_dx; a.lddx = lddx; a.rows = rows;
     a.weight = d_weight; a.bias = d_bias;

@@ -102,11 +102,3 @@ def test_native_caller_passes_doubles_and_many_integers():
     for wrong in ([1] * 25, [1.0] * 5, [1] * 30):
         with pytest.raises(TypeError):
             _lib.call()(address, *wrong)
-
-
-def test_numbers_that_are_no_integers_are_refused():
-    from accelgcn import _rows
-    assert _rows.mask_numbers(0, np.int64(5), 6, 7) == (0.0, 5, 6, 7)
-    for bad in ((0.5, 1.0, 0, 0), (0.5, 1, 0.5, 0), (0.5, 1, 0, 2.0)):
-        with pytest.raises(TypeError):
-            _rows.mask_numbers(*bad)

@@ -112,6 +112,13 @@ def test_many_rows(rows, cols, t):
     _case(rows, cols, t, relu=True, p=0.5, weight=True, bias=True)
 
 
+@pytest.mark.parametrize("rows,cols,t", [(1, 16, F32), (2, 4096, F32), (5, 3000, B16), (127, 16, F32), (129, 16, F32), (8192, 16, F32), (8193, 16, F32),
+                                         (2048, 60, F32), (2049, 60, F32), (2048, 61, F32), (1024, 128, F32), (1025, 128, F32), (2048, 128, B16), (2049, 128, B16),
+                                         (512, 255, F32), (64, 1000, F32), (65, 1000, F32), (64, 8192, B16), (65, 8191, F16), (8, 777, F32), (9, 777, F32)])
+def test_few_rows_whose_columns_one_cluster_adds_up(rows, cols, t):
+    _case(rows, cols, t, relu=True, p=0.25, weight=True, bias=True)
+
+
 def test_drawn_cases():
     rng = random.Random(20260)
     for _ in range(40):
