@@ -186,7 +186,8 @@ struct RowRing {
             copy_chunk(slot(k, j), from, bytes);
         }
     }
-    __device__ __forceinline__ void get(int k, int j, float *v) const { Elem<T>::unpack(load_shared(slot(k, j)), v); }
+    __device__ __forceinline__ uint4 get(int k, int j) const { return load_shared(slot(k, j)); }
+    __device__ __forceinline__ void get(int k, int j, float *v) const { Elem<T>::unpack(get(k, j), v); }
 };
 
 __device__ __forceinline__ float masked(float v, uint32_t bits) { return __uint_as_float(__float_as_uint(v) & bits); }
