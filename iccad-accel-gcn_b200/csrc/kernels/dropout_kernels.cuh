@@ -64,7 +64,7 @@ __device__ __forceinline__ void dropout_finish(const DropoutParams &p, int64_t o
                 for (int e = 0; e < E; e++) x[e] = relu_passes(g[e]) ? x[e] : 0.f;
             }
             if (WHOLE) *reinterpret_cast<uint4 *>(to[i + u]) = Elem<T>::pack(x);
-            else store_chunk<T, VEC, false>(to[i + u], -lo, hi - lo, x);
+            else store_chunk<T, VEC, false>(to[i + u], ((1u << hi) - 1) & ~((1u << lo) - 1), x);
         }
     }
 }
@@ -165,16 +165,19 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
             block[u] = (number >> 2) + u * words;
         }
         RowRing<T, TENSORS, U, STAGES> ring(s_ring);
-        const auto fetch = [&](int k) {
+        const auto fetch = [&](int k, bool near_first) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 if (k + u < turns) {
                     if (WHOLE) {
                         ring.fetch(0, u, v_from);
                         if (GATE) ring.fetch(TENSORS - 1, u, gate_from);
-                    } else {
+                    } else if (near_first) {
                         ring.fetch_edge(0, u, v_from, v_first, -lo, hi - lo, hi * (int)sizeof(T));
                         if (GATE) ring.fetch_edge(TENSORS - 1, u, gate_from, gate_first, -lo, hi - lo, hi * (int)sizeof(T));
+                    } else {
+                        ring.fetch(0, u, v_from, hi * (int)sizeof(T));
+                        if (GATE) ring.fetch(TENSORS - 1, u, gate_from, hi * (int)sizeof(T));
                     }
                 }
                 v_from += v_step;
@@ -184,7 +187,7 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
         };
         if (VEC) {
 #pragma unroll
-            for (int k = 0; k < STAGES; k++) { fetch(k * U); ring.next(); }
+            for (int k = 0; k < STAGES; k++) { fetch(k * U, true); ring.next(); }
         }
         for (int k = 0; k < turns; k += U) {
             uint4 v[U], gate[GATE ? U : 1];
@@ -195,7 +198,7 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
                     v[u] = ring.get(0, u);
                     if (GATE) gate[GATE ? u : 0] = ring.get(TENSORS - 1, u);
                 }
-                fetch(k + STAGES * U);
+                fetch(k + STAGES * U, false);
                 ring.next();
             } else {
                 float f[E];

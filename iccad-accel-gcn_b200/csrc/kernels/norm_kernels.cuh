@@ -21,8 +21,8 @@
 namespace agcn {
 
 constexpr int NORM_STAGES = 3;             // rows ahead in the ring
-// of the backward pass, one row per thread block: two tensors of 8192 columns and the weights are 192 KB in 32 bits, 160 KB in 16
-__host__ __device__ constexpr int norm_backward_stages(int lanes, int elem) { return lanes == 0 && elem == 4 ? 2 : NORM_STAGES; }
+// of the backward pass: with one row per thread block, two tensors of 8192 columns in 32 bits and the weights are 192 KB
+__host__ __device__ constexpr int norm_backward_stages(int lanes) { return lanes == 0 ? 2 : NORM_STAGES; }
 constexpr int NORM_THREADS = 256;          // of the forms with several rows per thread block
 constexpr int NORM_MAX_THREADS = 512;      // of the form with one: 8192 columns, 16 per thread
 static_assert(NORM_MAX_THREADS <= 32 * ROW_WARPS, "group_sum holds the sums of that many warps");
@@ -72,6 +72,7 @@ struct NormPlace {
     int turns, warp_turns;               // rows of the group; the most that a group of this warp has
     int shift;                           // elements that the group's rows begin behind a 16-byte boundary (LOOSE: taken as 0)
     uint32_t ok;                         // which of the thread's CH * E columns there are
+    int bytes[CH];                       // of its chunks in a ring, with what is in front of the row
     __device__ __forceinline__ NormPlace(const NormRows &part, const void *x, int64_t ldx, int cols)
     {
         lanes = L > 0 ? L : (int)blockDim.x;
@@ -88,32 +89,32 @@ struct NormPlace {
 #pragma unroll
             for (int e = 0; e < E; e++)
                 if (column(j) + e >= 0 && column(j) + e < cols) ok |= 1u << (j * E + e);
+#pragma unroll
+        for (int j = 0; j < CH; j++) bytes[j] = cols - column(j) >= E ? 16 : (cols - column(j)) * (int)sizeof(T);
     }
     __device__ __forceinline__ int column(int j) const { return (j * lanes + t) * E - shift; }
     // All ones where the thread has the column (WHOLE: a chunk is there or not; a slot of the ring that is never filled is 0)
     __device__ __forceinline__ uint32_t mine(int j, int e) const { return 0u - (ok >> (j * E + (LAYOUT == ROWS_WHOLE ? 0 : e)) & 1u); }
     __device__ __forceinline__ bool has(int j) const { return ok >> (j * E) & ((1u << E) - 1); }
-    // Starts the copies of a row's chunks, from where this thread's first one is.
+    // Starts the copies of a row's chunks, from where this thread's first one is (near_first: the row may be one of the first few).
     template <int N, int STAGES>
-    __device__ __forceinline__ void fetch(const RowRing<T, N, CH, STAGES> &ring, int k, const T *from, const T *first, int cols) const
+    __device__ __forceinline__ void fetch(const RowRing<T, N, CH, STAGES> &ring, int k, const T *from, const T *first, int cols, bool near_first) const
     {
 #pragma unroll
         for (int j = 0; j < CH; j++) {
             if (!has(j)) continue;
             if (LAYOUT == ROWS_WHOLE) ring.fetch(k, j, from + j * lanes * E);
-            else {
-                const int n = cols - column(j);
-                ring.fetch_edge(k, j, from + j * lanes * E, first, column(j), cols, n >= E ? 16 : n * (int)sizeof(T));
-            }
+            else if (near_first) ring.fetch_edge(k, j, from + j * lanes * E, first, column(j), cols, bytes[j]);
+            else ring.fetch(k, j, from + j * lanes * E, bytes[j]);
         }
     }
     // Stores a row's chunks, to where this thread's first one is.
     template <bool VEC>
-    __device__ __forceinline__ void store(T *to, int cols, const float (&v)[CH][E]) const
+    __device__ __forceinline__ void store(T *to, const float (&v)[CH][E]) const
     {
 #pragma unroll
         for (int j = 0; j < CH; j++)
-            if (has(j)) store_chunk<T, VEC, LAYOUT == ROWS_WHOLE>(to + j * lanes * E, column(j), cols, v[j]);
+            if (has(j)) store_chunk<T, VEC, LAYOUT == ROWS_WHOLE>(to + j * lanes * E, ok >> (j * E) & ((1u << E) - 1), v[j]);
     }
 };
 
@@ -157,15 +158,19 @@ __device__ __forceinline__ float inverse_sqrt(float v)
 template <int CH, int E>
 __device__ __forceinline__ void drop(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, float (&v)[CH][E])
 {
-    int64_t blocks[CH];
-    uint32_t word[CH][E];
+    constexpr int AT_ONCE = CH > 1 ? CH / 2 : 1;             // half of them at once: all take the registers of a third of the warps
 #pragma unroll
-    for (int j = 0; j < CH; j++) blocks[j] = block + j * stride;
-    draw_words<CH, E>(m, offset, blocks, skip, word);
+    for (int i = 0; i < CH; i += AT_ONCE) {
+        int64_t blocks[AT_ONCE];
+        uint32_t word[AT_ONCE][E];
 #pragma unroll
-    for (int j = 0; j < CH; j++)
+        for (int j = 0; j < AT_ONCE; j++) blocks[j] = block + (i + j) * stride;
+        draw_words<AT_ONCE, E>(m, offset, blocks, skip, word);
 #pragma unroll
-        for (int e = 0; e < E; e++) v[j][e] = word[j][e] >= m.threshold ? v[j][e] : 0.f;
+        for (int j = 0; j < AT_ONCE; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[i + j][e] = word[j][e] >= m.threshold ? v[i + j][e] : 0.f;
+    }
 }
 
 __device__ __forceinline__ float sum4(const float2 (&v)[2])
@@ -192,14 +197,15 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
     const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols);
 
     extern __shared__ uint4 s_ring[];
-    RowRing<T, 1, CH, NORM_STAGES> ring(s_ring);
+    constexpr int STAGES = NORM_STAGES;
+    RowRing<T, 1, CH, STAGES> ring(s_ring);
     wait_for_predecessor();
     const T *const first = static_cast<const T *>(p.x), *x = first + at.group * p.ldx + at.column(0);
     if (VEC) {
 #pragma unroll
-        for (int k = 0; k < NORM_STAGES; k++) {
+        for (int k = 0; k < STAGES; k++) {
             ring.clear();
-            if (k < at.turns) at.fetch(ring, 0, x, first, cols);
+            if (k < at.turns) at.fetch(ring, 0, x, first, cols, true);
             commit_copies();
             ring.next();
             x += p.x_step;
@@ -233,10 +239,10 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         float one[1], two[2];
         float2 part[3][2] = {};
         if (VEC) {
-            wait_copies<NORM_STAGES - 1>();
+            wait_copies<STAGES - 1>();
 #pragma unroll
             for (int j = 0; j < CH; j++) ring.get(0, j, d[j]);
-            if (k + NORM_STAGES < at.turns) at.fetch(ring, 0, x, first, cols);
+            if (k + STAGES < at.turns) at.fetch(ring, 0, x, first, cols, false);
             commit_copies();
             ring.next();
         } else {
@@ -291,7 +297,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
         }
         if (live) {
             if (p.stats != nullptr && at.t == 0) *stats = make_float2(m + off, s);
-            at.template store<VEC>(y, cols, d);
+            at.template store<VEC>(y, d);
         }
         y += p.y_step;
         stats += at.groups;
@@ -331,7 +337,7 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
     const NormPlace<T, L, CH, LAYOUT> at(p.part, p.x, p.ldx, cols);
 
     extern __shared__ uint4 s_ring[];
-    constexpr int STAGES = norm_backward_stages(L, E);
+    constexpr int STAGES = norm_backward_stages(L);
     RowRing<T, 2, CH, STAGES> ring(s_ring);
     wait_for_predecessor();
     const T *const x_first = static_cast<const T *>(p.x), *const dy_first = static_cast<const T *>(p.dy);
@@ -341,8 +347,8 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
         for (int k = 0; k < STAGES; k++) {
             ring.clear();
             if (k < at.turns) {
-                at.fetch(ring, 0, x, x_first, cols);
-                at.fetch(ring, 1, dy, dy_first, cols);
+                at.fetch(ring, 0, x, x_first, cols, true);
+                at.fetch(ring, 1, dy, dy_first, cols, true);
             }
             commit_copies();
             ring.next();
@@ -398,8 +404,8 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
                 ring.get(1, j, g[j]);
             }
             if (k + STAGES < at.turns) {
-                at.fetch(ring, 0, x, x_first, cols);
-                at.fetch(ring, 1, dy, dy_first, cols);
+                at.fetch(ring, 0, x, x_first, cols, false);
+                at.fetch(ring, 1, dy, dy_first, cols, false);
             }
             commit_copies();
             ring.next();
@@ -481,7 +487,7 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
             for (int j = 0; j < CH; j++)
 #pragma unroll
                 for (int e = 0; e < E; e += 2) unpair(fma2(pair(&h[j][e]), both(-m2), fma2(pair(&g[j][e]), both(s), both(-m1))), &g[j][e]);
-            at.template store<VEC>(dx, cols, g);
+            at.template store<VEC>(dx, g);
         }
         dx += p.dx_step;
         block += p.part.words;

@@ -117,16 +117,16 @@ __device__ __forceinline__ void load_chunk(const T *row, int c0, int cols, float
         for (int e = 0; e < E; e++) v[e] = c0 + e >= 0 && c0 + e < cols ? Elem<T>::get(row[c0 + e]) : 0.f;
     }
 }
-// The same into memory; `to`: where column c0 goes (in front of the row for c0 < 0).  WHOLE: the chunk is known to be whole.
+// The same into memory, to `to` on: the elements whose bits are set.  WHOLE: all of them are known to be.
 template <typename T, bool VEC, bool WHOLE>
-__device__ __forceinline__ void store_chunk(T *to, int c0, int cols, const float *v)
+__device__ __forceinline__ void store_chunk(T *to, uint32_t bits, const float *v)
 {
     constexpr int E = Elem<T>::E;
-    if (VEC && (WHOLE || (c0 >= 0 && c0 + E <= cols))) {
+    if (VEC && (WHOLE || bits == (1u << E) - 1)) {
         *reinterpret_cast<uint4 *>(to) = Elem<T>::pack(v);
     } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) if (c0 + e >= 0 && c0 + e < cols) to[e] = Elem<T>::put(v[e]);
+        for (int e = 0; e < E; e++) if (bits >> e & 1u) to[e] = Elem<T>::put(v[e]);
     }
 }
 
@@ -174,8 +174,10 @@ struct RowRing {
     }
     // Starts the copy of chunk j of tensor k: of a whole one at `from`, ...
     __device__ __forceinline__ void fetch(int k, int j, const T *from) const { copy_chunk(slot(k, j), from); }
-    // ... or of `bytes` of it, elements c0 .. of a row: what is in front of the row within its first 16 bytes comes along, unused;
-    // nothing in front of the tensor, at `first`, or behind the row is read.
+    // ... or of `bytes` of it: what is in front of the row within its first 16 bytes comes along, unused, ...
+    __device__ __forceinline__ void fetch(int k, int j, const T *from, int bytes) const { copy_chunk(slot(k, j), from, bytes); }
+    // ... but not where that would be in front of the tensor, at `first` (the chunk has elements c0 .. of a row; only the first few rows
+    // can be that near).
     __device__ __forceinline__ void fetch_edge(int k, int j, const T *from, const T *first, int c0, int cols, int bytes) const
     {
         if (from < first) {
@@ -183,7 +185,7 @@ struct RowRing {
             load_chunk<T, false>(from - c0, c0, cols, v);
             store_shared(slot(k, j), Elem<T>::pack(v));
         } else {
-            copy_chunk(slot(k, j), from, bytes);
+            fetch(k, j, from, bytes);
         }
     }
     __device__ __forceinline__ uint4 get(int k, int j) const { return load_shared(slot(k, j)); }

@@ -7,12 +7,12 @@ namespace agcn {
 
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
-constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8, NORM_EDGE_ELEMS = 8;
+constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
 // Backward pass: a call whose groups would have up to NORM_CLUSTER_TURNS rows in turn runs as one cluster of up to NORM_CLUSTER thread
 // blocks, which adds up the columns itself.  2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace.
 constexpr int NORM_CLUSTER = 8, NORM_CLUSTER_TURNS = 8;
 constexpr int NORM_MAX_SMEM = 200 * 1024;
-static_assert(NORM_MAX_THREADS * NORM_ELEMS * (norm_backward_stages(0, 4) * 2 * 4 + 8) <= NORM_MAX_SMEM, "8192 columns in 32 bits");
+static_assert(NORM_MAX_THREADS * NORM_ELEMS * (norm_backward_stages(0) * 2 * 4 + 8) <= NORM_MAX_SMEM, "8192 columns in 32 bits");
 
 struct NormForm {
     int layout;                             // RowLayout
@@ -33,7 +33,6 @@ inline NormForm norm_form_of(int layout, int64_t cols, int dtype, int per_lane, 
     if (cols + shift > NORM_MAX_COLS) f.layout = ROWS_LOOSE;
     if (f.layout == ROWS_LOOSE) shift = 0;
     const int chunks = (int)ceil_div(cols + shift, e);
-    if (f.layout == ROWS_EDGES && per_lane > NORM_EDGE_ELEMS) per_lane = NORM_EDGE_ELEMS;
     f.lanes = 2;
     while (f.lanes < 32 && f.lanes * per_lane / e < chunks) f.lanes *= 2;
     f.threads = NORM_THREADS;
@@ -100,7 +99,7 @@ template <typename F> int norm_dispatch(const NormForm &f, int dtype, F &&launch
 // row, weight and bias of the backward pass
 inline int norm_smem(const NormForm &f, int tensors, int elems)
 {
-    const int stages = tensors == 2 ? norm_backward_stages(f.lanes, elems) : NORM_STAGES;
+    const int stages = tensors == 2 ? norm_backward_stages(f.lanes) : NORM_STAGES;
     return f.threads * f.chunks * (stages * tensors * 16 + (f.lanes == 0 && tensors == 2 ? 8 * elems : 0));
 }
 
