@@ -5,6 +5,7 @@ A call on a graph of a few thousand nodes takes 3 us on the GPU; every attribute
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -47,14 +48,12 @@ def more_features(name, t, rows, cols, dtype, dev):
     return ld
 
 
-def array(name, t, shape, dev):
-    """Address of a contiguous float32 array on the features' device (None where there is none)."""
-    if t is None:
-        return None
+def array(name, t, count, dev):
+    """Address of a contiguous float32 array of `count` elements on the features' device."""
     if t.dtype is not F32 or t.get_device() != dev:
         raise TypeError(f"{name} must be a float32 tensor on the features' device")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {list(shape)}")
+    if t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, of {count} elements")
     return t.data_ptr()
 
 
@@ -78,25 +77,7 @@ def empty(rows, cols, dtype, dev, stream):
         return torch.empty((rows, cols), dtype=dtype, device=f"cuda:{dev}")
 
 
-_address = {}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_call = None
-
-
-def run(function, dev, stream, *args):
-    """The library's `function` on device `dev`, its last argument the stream (None: the current one)."""
-    global _call
-    if _call is None:
-        _lib.load()
-        _call = _lib.call()
-    address = _address.get(function)
-    if address is None:
-        address = _address[function] = _lib.address(function)
-    s = _raw_stream(dev) if stream is None else stream.cuda_stream
-    if torch._C._cuda_getDevice() == dev:
-        rc = _call(address, *args, s)
-    else:
-        with torch.cuda.device(dev):
-            rc = _call(address, *args, s)
-    if rc != 0:
-        _lib.check(rc)
+def function(name):
+    """The library's function: called with its arguments, it returns its status."""
+    _lib.load()
+    return functools.partial(_lib.call(), _lib.address(name))

@@ -19,6 +19,10 @@ import torch
 
 from . import _lib, _rows
 
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_forward = _backward = None
+
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, relu: bool = False, p: float = 0.0, seed: int = 0, offset: int = 0,
                row0: int = 0, step=None, out=None, stats=None, stream=None):
@@ -27,23 +31,31 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, relu: bool = False,
     [rows, 2], receives mean and 1 / sqrt(variance + eps) of the rows: what the backward pass needs.  row0: where this
     rank's rows begin in the whole.  step: an int64 on the device that is added to `offset` when the kernel runs (a captured
     graph counts it up to have new masks).  out may be x.  Asynchronous on the current stream (or `stream`)."""
+    global _forward
     rows, cols, ldx, code, dtype, dev = _rows.features("x", x)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return layer_norm(x, weight, bias, eps, relu, p, seed, offset, row0, step, out, stats, stream)
+    if _forward is None:
+        _forward = _rows.function("agcn_layer_norm")
     if out is None:
         out, ldy = _rows.empty(rows, cols, dtype, dev, stream), cols
     else:
         ldy = _rows.more_features("out", out, rows, cols, dtype, dev)
-    vector = (cols,)
-    _rows.run("agcn_layer_norm", dev, stream, x.data_ptr(), ldx, _rows.array("weight", weight, vector, dev), _rows.array("bias", bias, vector, dev),
-              float(eps), out.data_ptr(), ldy, None if stats is None else _rows.array("stats", stats, (rows, 2), dev), rows, cols, code,
-              1 if relu else 0, float(p), index(seed), index(offset), None if step is None else _rows.step_address(step, dev), index(row0))
+    rc = _forward(x.data_ptr(), ldx, None if weight is None else _rows.array("weight", weight, cols, dev),
+                  None if bias is None else _rows.array("bias", bias, cols, dev), float(eps), out.data_ptr(), ldy,
+                  None if stats is None else _rows.array("stats", stats, 2 * rows, dev), rows, cols, code, 1 if relu else 0, float(p), index(seed),
+                  index(offset), None if step is None else _rows.step_address(step, dev), index(row0),
+                  _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if rc != 0:
+        _lib.check(rc)
     return out
 
 
 @functools.lru_cache(maxsize=4096)
 def _work_floats(dev: int, rows: int, cols: int, dtype: int) -> int:
     n = ctypes.c_int64()
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().agcn_layer_norm_backward_work(rows, cols, dtype, ctypes.byref(n)))
+    _lib.check(_lib.load().agcn_layer_norm_backward_work(rows, cols, dtype, ctypes.byref(n)))      # of the current device: `dev`
     return n.value // 4
 
 
@@ -52,7 +64,13 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None, relu: bool = False
     """Gradients of `layer_norm`: (dx, dweight, dbias) from dy, and the x, stats, weight, bias and mask numbers of the forward
     pass.  dweight and dbias are float32 [cols], overwritten, the same bits from run to run; None where there was no weight (bias)
     and no array is given for it.  dx may be dy or x.  Asynchronous on the current stream (or `stream`)."""
+    global _backward
     rows, cols, ldx, code, dtype, dev = _rows.features("x", x)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return layer_norm_backward(dy, x, stats, weight, bias, relu, p, seed, offset, row0, step, dx, dweight, dbias, stream)
+    if _backward is None:
+        _backward = _rows.function("agcn_layer_norm_backward")
     lddy = _rows.more_features("dy", dy, rows, cols, dtype, dev)
     if stats is None:
         raise TypeError("layer_norm_backward needs the stats of the forward pass")
@@ -73,10 +91,12 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None, relu: bool = False
             # of this call alone: calls on other streams, and captured graphs, have their own
             with _rows.allocating_on(stream):
                 work = torch.empty(n, dtype=_rows.F32, device=x.device)
-    vector = (cols,)
-    _rows.run("agcn_layer_norm_backward", dev, stream, dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.array("stats", stats, (rows, 2), dev),
-              _rows.array("weight", weight, vector, dev), _rows.array("bias", bias, vector, dev), dx.data_ptr(), lddx,
-              _rows.array("dweight", dweight, vector, dev), _rows.array("dbias", dbias, vector, dev), None if work is None else work.data_ptr(), 4 * n,
-              rows, cols, code, 1 if relu else 0, float(p), index(seed), index(offset), None if step is None else _rows.step_address(step, dev),
-              index(row0))
+    rc = _backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.array("stats", stats, 2 * rows, dev),
+                   None if weight is None else _rows.array("weight", weight, cols, dev), None if bias is None else _rows.array("bias", bias, cols, dev),
+                   dx.data_ptr(), lddx, None if dweight is None else _rows.array("dweight", dweight, cols, dev),
+                   None if dbias is None else _rows.array("dbias", dbias, cols, dev), None if work is None else work.data_ptr(), 4 * n, rows, cols, code,
+                   1 if relu else 0, float(p), index(seed), index(offset), None if step is None else _rows.step_address(step, dev), index(row0),
+                   _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if rc != 0:
+        _lib.check(rc)
     return dx, dweight, dbias
