@@ -23,6 +23,7 @@ namespace agcn {
 constexpr int NORM_STAGES = 3;             // rows ahead in the ring
 // of the backward pass: with one row per thread block, two tensors of 8192 columns in 32 bits and the weights are 192 KB
 __host__ __device__ constexpr int norm_backward_stages(int lanes) { return lanes == 0 ? 2 : NORM_STAGES; }
+constexpr int NORM_CLUSTER = 8;            // thread blocks of a backward pass that are one cluster, at most
 constexpr int NORM_THREADS = 256;          // of the forms with several rows per thread block
 constexpr int NORM_MAX_THREADS = 512;      // of the form with one: 8192 columns, 16 per thread
 static_assert(NORM_MAX_THREADS <= 32 * ROW_WARPS, "group_sum holds the sums of that many warps");
@@ -96,6 +97,19 @@ struct NormPlace {
     // All ones where the thread has the column (WHOLE: a chunk is there or not; a slot of the ring that is never filled is 0)
     __device__ __forceinline__ uint32_t mine(int j, int e) const { return 0u - (ok >> (j * E + (LAYOUT == ROWS_WHOLE ? 0 : e)) & 1u); }
     __device__ __forceinline__ bool has(int j) const { return ok >> (j * E) & ((1u << E) - 1); }
+    // The thread's columns of a per-column array (null: `none` in all of them), `missing` where there are none: all loads under way at once.
+    __device__ __forceinline__ void load_columns(const float *from, float none, float missing, float (&v)[CH][E]) const
+    {
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[j][e] = ok >> (j * E + e) & 1u ? none : missing;
+        if (from == nullptr) return;
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) if (ok >> (j * E + e) & 1u) v[j][e] = from[column(j) + e];
+    }
     // Starts the copies of a row's chunks, from where this thread's first one is (near_first: the row may be one of the first few).
     template <int N, int STAGES>
     __device__ __forceinline__ void fetch(const RowRing<T, N, CH, STAGES> &ring, int k, const T *from, const T *first, int cols, bool near_first) const
@@ -214,16 +228,16 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
 
     float w[CH][E], b[CH][E];
     uint32_t own[CH][E];
+    at.load_columns(p.weight, 1.f, 1.f, w);
+    at.load_columns(p.bias, 0.f, 0.f, b);
+    // the mask's factor is in them: what is kept is multiplied by it, and it is positive
+    const float scale = p.mask.on ? p.mask.scale : 1.f;
 #pragma unroll
     for (int j = 0; j < CH; j++)
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int c = at.column(j) + e;
-            const bool in = c >= 0 && c < cols;
-            // the mask's factor is in them: what is kept is multiplied by it, and it is positive
-            const float scale = p.mask.on ? p.mask.scale : 1.f;
-            w[j][e] = in && p.weight != nullptr ? p.weight[c] * scale : scale;
-            b[j][e] = in && p.bias != nullptr ? p.bias[c] * scale : 0.f;
+            w[j][e] *= scale;
+            b[j][e] *= scale;
             own[j][e] = at.mine(j, e);
         }
     const int64_t offset = mask_offset(p.mask);
@@ -370,7 +384,7 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
             const int c = at.column(j) + e;
             const bool in = c >= 0 && c < cols;
             wj[e] = in && p.weight != nullptr ? p.weight[c] : 1.f;
-            bj[e] = !in ? INFINITY : p.bias != nullptr ? p.bias[c] : 0.f;       // a column that is not there is never near zero
+            bj[e] = !in ? INFINITY : p.bias != nullptr ? p.bias[c] : 0.f;         // a column that is not there is never near zero
             // z = h w + b is off by less than 2^-22 |b| where the two terms cancel: its sign is not certain below that
             if (in) uncertain = fmaxf(uncertain, fabsf(bj[e]) * 4.76837158e-7f);
             sum_w[j][e] = sum_b[j][e] = 0.f;
@@ -524,34 +538,46 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
         for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < 2 * cols; c += gridDim.x * blockDim.x) {
             float *out = c < cols ? p.dweight : p.dbias;
             if (out == nullptr) continue;
-            float s = 0.f;
-            for (unsigned k = 0; k < gridDim.x; k++) s += *cluster.map_shared_rank(s_parts + c, k);
+            float s = 0.f, v[NORM_CLUSTER];
+#pragma unroll
+            for (int k = 0; k < NORM_CLUSTER; k++) v[k] = k < (int)gridDim.x ? *cluster.map_shared_rank(s_parts + c, k) : 0.f;
+#pragma unroll
+            for (int k = 0; k < NORM_CLUSTER; k++) s += v[k];
             out[c < cols ? c : c - cols] = s;
         }
         cluster.sync();                        // nobody leaves while its sums are read
     }
 }
 
-// Column sums of the thread blocks' rows: 32 columns per thread block, its 8 warps over the rows in turn.
-static __global__ void __launch_bounds__(256)
-norm_columns_kernel(const float *__restrict__ parts, int64_t part_stride, int n_parts, float *__restrict__ dweight, float *__restrict__ dbias, int cols)
+// Column sums of the thread blocks' rows: 32 columns per thread block, its 32 warps over the rows in turn, 8 of them under way.
+static __global__ void __launch_bounds__(1024)
+norm_columns_kernel(const float *parts, int64_t part_stride, int n_parts, float *__restrict__ dweight, float *__restrict__ dbias, int cols)
 {
-    __shared__ float s_sum[8][33];
+    __shared__ float s_sum[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float *out = blockIdx.y == 0 ? dweight : dbias;
     if (out == nullptr) return;
     wait_for_predecessor();
     float s = 0.f;
-    if (c < cols)
-        for (int k = warp; k < n_parts; k += 8) s += parts[k * part_stride + (int64_t)blockIdx.y * cols + c];
+    if (c < cols) {
+        const float *from = parts + (int64_t)blockIdx.y * cols + c;
+        int k = warp;
+        for (; k + 7 * 32 < n_parts; k += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = from[(k + u * 32) * part_stride];
+#pragma unroll
+            for (int u = 0; u < 8; u++) s += v[u];
+        }
+#pragma unroll 8
+        for (; k < n_parts; k += 32) s += from[k * part_stride];
+    }
     s_sum[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < cols) {
-        s = 0.f;
+    s = s_sum[lane][warp];                     // lane: the warp that made it; warp: the column
 #pragma unroll
-        for (int k = 0; k < 8; k++) s += s_sum[k][lane];
-        out[c] = s;
-    }
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane == 0 && blockIdx.x * 32 + warp < cols) out[blockIdx.x * 32 + warp] = s;
 }
 
 }  // namespace agcn

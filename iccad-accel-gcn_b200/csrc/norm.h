@@ -8,9 +8,10 @@ namespace agcn {
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
 constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
-// Backward pass: a call whose groups would have up to NORM_CLUSTER_TURNS rows in turn runs as one cluster of up to NORM_CLUSTER thread
-// blocks, which adds up the columns itself.  2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace.
-constexpr int NORM_CLUSTER = 8, NORM_CLUSTER_TURNS = 8;
+// Backward pass: a call whose groups would have up to so many rows in turn runs as one cluster, which adds up the columns itself: 8 where a
+// row is a group's within a warp (2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace), 2 where it takes a thread
+// block (64 rows of 8 192: 29 us as 8 turns of 8, 19 as 64 thread blocks and a second kernel).
+constexpr int NORM_CLUSTER_TURNS = 8, NORM_CLUSTER_WIDE_TURNS = 2;
 constexpr int NORM_MAX_SMEM = 200 * 1024;
 static_assert(NORM_MAX_THREADS * NORM_ELEMS * (norm_backward_stages(0) * 2 * 4 + 8) <= NORM_MAX_SMEM, "8192 columns in 32 bits");
 

@@ -7,7 +7,7 @@ namespace agcn {
 static bool norm_one_cluster(int64_t rows, int64_t cols, int dtype)
 {
     const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
-    return rows <= NORM_CLUSTER * NORM_CLUSTER_TURNS * f.rows_per_block;
+    return rows <= NORM_CLUSTER * (f.lanes > 0 ? NORM_CLUSTER_TURNS : NORM_CLUSTER_WIDE_TURNS) * f.rows_per_block;
 }
 
 // Thread blocks whose sums the workspace holds: all that are resident, for the forms there are
@@ -15,7 +15,10 @@ static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int sms)
 {
     if (norm_one_cluster(rows, cols, dtype)) return 0;
     const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
-    const int64_t most = sms * (2048 / f.threads);
+    // What a thread block writes for its columns (8 bytes each) should be little beside the rows that it reads: 16 of them at
+    // least, but two thread blocks per SM where there are few rows.
+    const int64_t resident = sms * (2048 / f.threads), few = 2 * sms > rows / 16 ? 2 * sms : rows / 16;
+    const int64_t most = few < resident ? few : resident;
     return rows < most ? rows : most;
 }
 
@@ -38,7 +41,7 @@ struct NormBackwardLaunch {
         if (wanted && most_parts == 0) {
             const int64_t needed = ceil_div(p.rows, f.rows_per_block);
             for (grid = 1; grid < needed && grid < NORM_CLUSTER; grid *= 2) {}
-            p.cluster = 1;
+            p.cluster = grid > 1;              // alone, a thread block's sums are the sums
         } else if (wanted) {
             grid = norm_grid(f, p.rows, resident < most_parts ? resident : most_parts);
             p.part_stride = 2 * p.cols;
@@ -59,8 +62,8 @@ struct NormBackwardLaunch {
         cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(f.threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
         cfg.attrs = attr; cfg.numAttrs = p.cluster ? 2 : 1;
         AGCN_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-        if (wanted && !p.cluster)
-            AGCN_CUDA(launch_early(true, norm_columns_kernel, dim3((unsigned)ceil_div(p.cols, 32), 2), 256, 0, s, work, p.part_stride, (int)grid, dweight,
+        if (wanted && most_parts > 0)
+            AGCN_CUDA(launch_early(true, norm_columns_kernel, dim3((unsigned)ceil_div(p.cols, 32), 2), 1024, 0, s, work, p.part_stride, (int)grid, dweight,
                                    dbias, p.cols));
         return AGCN_OK;
     }

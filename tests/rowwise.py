@@ -78,9 +78,9 @@ def backward(dy, x, stats, w, b, relu, p, keep):
     dx = rstd * (g - m1 - h * m2)
     # g: 3 roundings, h: 2; the means 41 of a sum and up to 6 before it; 4 at the end
     off = 56 * U * rstd * (g.abs() + g.abs().mean(1, keepdim=True) + h.abs() * (g * h).abs().mean(1, keepdim=True))
-    # a column: a thread's rows in turn (fewer than 512 in these tests), up to 64 groups of a thread block, the blocks by
-    # eighths (up to 148 in turn) and the 8 of those, and 5 before the sum
-    deep = min(rows, 512) + 64 + 148 + 8 + 5
+    # a column: a thread's rows in turn (fewer than 512 in these tests), up to 128 groups of a thread block, the blocks by
+    # 32nds (up to 148 in turn) and 5 exchanges of those, and 5 before the sum
+    deep = min(rows, 512) + 128 + 148 + 5 + 5
     return {"dx": (dx, off + rounding(dx, off, t)), "dweight": ((dz * h).sum(0), deep * U * (dz * h).abs().sum(0)),
             "dbias": (dz.sum(0), deep * U * dz.abs().sum(0))}
 

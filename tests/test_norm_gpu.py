@@ -411,7 +411,7 @@ def test_elements_beyond_32_bits():
         h = (x[part].double() - stats[part, :1].double()) * stats[part, 1:].double()
         dz = torch.where(y[part] > 0, y[part].double() * 2, 0.0)
         dw64 += (dz * h).sum(0); db64 += dz.sum(0); aw += (dz * h).abs().sum(0); ab += dz.abs().sum(0)
-    deep = 14_400 + 64 + 148 + 8 + 5
+    deep = 14_400 + 128 + 148 + 5 + 5
     # (an output that rounds to 0 in 16 bits though z > 0 has dy = 0 and adds nothing)
     rowwise.check("dweight", dw, dw64, deep * rowwise.U * aw)
     rowwise.check("dbias", db, db64, deep * rowwise.U * ab)
