@@ -57,6 +57,13 @@ def array(name, t, count, dev):
     return t.data_ptr()
 
 
+def stats(name, t, rows, dev):
+    """Address of the rows' statistics [rows, 2]."""
+    if t.shape != (rows, 2):
+        raise ValueError(f"{name} must be [{rows}, 2]")
+    return array(name, t, 2 * rows, dev)
+
+
 def step_address(step, dev):
     """Address of the device counter that is added to a mask's offset."""
     if step.dtype is not torch.int64 or step.get_device() != dev or step.numel() != 1:

@@ -7,7 +7,7 @@ of agcn_layer_norm / agcn_layer_norm_backward.
     dy, dweight, dbias = norm.layer_norm_backward(dh, y, stats, weight, bias, relu=True, p=0.5, seed=seed, offset=step)
 
 One pass over the rows each.  The dropout mask is made from (seed, offset, the element's number) in both and never stored:
-give every layer and step another offset, and both passes of one the same.
+give every layer and step another offset, and both passes of one the same.  These are plain functions on tensors: autograd does not see them.
 """
 from __future__ import annotations
 
@@ -44,7 +44,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, relu: bool = False,
         ldy = _rows.more_features("out", out, rows, cols, dtype, dev)
     rc = _forward(x.data_ptr(), ldx, None if weight is None else _rows.array("weight", weight, cols, dev),
                   None if bias is None else _rows.array("bias", bias, cols, dev), float(eps), out.data_ptr(), ldy,
-                  None if stats is None else _rows.array("stats", stats, 2 * rows, dev), rows, cols, code, 1 if relu else 0, float(p), index(seed),
+                  None if stats is None else _rows.stats("stats", stats, rows, dev), rows, cols, code, 1 if relu else 0, float(p), index(seed),
                   index(offset), None if step is None else _rows.step_address(step, dev), index(row0),
                   _raw_stream(dev) if stream is None else stream.cuda_stream)
     if rc != 0:
@@ -91,7 +91,7 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None, relu: bool = False
             # of this call alone: calls on other streams, and captured graphs, have their own
             with _rows.allocating_on(stream):
                 work = torch.empty(n, dtype=_rows.F32, device=x.device)
-    rc = _backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.array("stats", stats, 2 * rows, dev),
+    rc = _backward(dy.data_ptr(), lddy, x.data_ptr(), ldx, _rows.stats("stats", stats, rows, dev),
                    None if weight is None else _rows.array("weight", weight, cols, dev), None if bias is None else _rows.array("bias", bias, cols, dev),
                    dx.data_ptr(), lddx, None if dweight is None else _rows.array("dweight", dweight, cols, dev),
                    None if dbias is None else _rows.array("dbias", dbias, cols, dev), None if work is None else work.data_ptr(), 4 * n, rows, cols, code,

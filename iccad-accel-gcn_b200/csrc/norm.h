@@ -7,6 +7,8 @@ namespace agcn {
 
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
+// Elements of a row per lane that a group within a warp aims at: 16 forward (with 8, 47 instructions per element in place of 29: 600 us for
+// 2 400 000 x 128 in place of 435); 8 backward, where 16 take over 200 registers.
 constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
 // Backward pass: a call whose groups would have up to so many rows in turn runs as one cluster, which adds up the columns itself: 8 where a
 // row is a group's within a warp (2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace), 2 where it takes a thread

@@ -1,5 +1,6 @@
 // Gradients of layer norm, ReLU and dropout (norm.cu) in one pass over the rows, and the column sums.
 #include "norm.h"
+#include "kernels/norm_backward_kernels.cuh"
 
 namespace agcn {
 

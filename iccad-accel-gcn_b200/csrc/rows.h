@@ -10,6 +10,7 @@
 namespace agcn {
 
 constexpr int64_t ROWS_MAX_ELEMENTS = (int64_t)1 << 60;       // numbers of elements, their strides and the mask's counters stay in 64 bits
+constexpr int64_t ROWS_MAX_STRIDE = (int64_t)1 << 40;          // times the groups of a launch, too
 
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline int dtype_bytes(int dtype) { return dtype == AGCN_F32 ? 4 : 2; }
@@ -26,7 +27,7 @@ inline int check_rows(const char *who, const Rows &t, int64_t rows, int64_t cols
     AGCN_REQUIRE(t.ptr != nullptr, "%s: %s is null", who, t.name);
     AGCN_REQUIRE(reinterpret_cast<uintptr_t>(t.ptr) % dtype_bytes(dtype) == 0, "%s: %s is not aligned to its elements", who, t.name);
     AGCN_REQUIRE(t.ld >= cols, "%s: rows of %s are %lld elements apart, fewer than the %lld columns", who, t.name, (long long)t.ld, (long long)cols);
-    AGCN_REQUIRE(t.ld <= ROWS_MAX_ELEMENTS / rows, "%s: row stride of %s out of range", who, t.name);
+    AGCN_REQUIRE(t.ld <= ROWS_MAX_STRIDE && t.ld <= ROWS_MAX_ELEMENTS / rows, "%s: row stride of %s out of range", who, t.name);
     return AGCN_OK;
 }
 

@@ -451,7 +451,9 @@ int agcn_gcn2_forward_destroy(agcn_gcn2 *fwd);
  * others element by element; between layouts, sums may be made in another order).  Statistics, sums, weights and their gradients are fp32, and
  * so is all arithmetic; a result is rounded to `dtype` once.  An output may be an input of the same call with the
  * same stride (y = x, dx = dy or x); other overlaps are not allowed.  All calls are asynchronous on `stream`,
- * allocate nothing and may be captured.  rows = 0 is allowed.
+ * allocate nothing and may be captured (the first call of a form on a device loads its kernel: make it before).
+ * rows = 0 is allowed.  Launches start early behind the one before them on the stream (programmatic dependent
+ * launch) and wait for its end before they touch memory.
  * AGCN_ACT_RELU: max(., 0); NaN stays NaN here (so a broken step shows), its gradient passes.
  *
  * Dropout: 0 <= p < 1.  Element (r, c) has the number i = (row0 + r) * cols + c and is kept if word i % 4 of
@@ -478,7 +480,7 @@ int agcn_layer_norm(const void *d_x, int64_t ldx, const float *d_weight, const f
 /* Its gradients, from dy, the x, stats, weight and bias of the forward pass, and the same activation and mask:
  * d_dx [rows x cols] of `dtype`, d_dweight and d_dbias [cols] fp32 (overwritten; either may be NULL).  The sums over
  * the rows are made in one order: the same bits from run to run on one GPU model.  d_work: fp32 workspace of at least
- * agcn_layer_norm_backward_work(...) bytes (what the current device needs), whose contents mean nothing before and
+ * agcn_layer_norm_backward_work(...) bytes (what the current device needs; 0 for few rows), whose contents mean nothing before and
  * after; calls that may overlap need one each.  NULL where neither d_dweight nor d_dbias is wanted. */
 int agcn_layer_norm_backward_work(int64_t rows, int64_t cols, int dtype, int64_t *bytes);
 int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const float *d_stats,

@@ -42,7 +42,7 @@ BAD = [(f, k, v, word) for f in ("agcn_layer_norm", "agcn_layer_norm_backward", 
                           ("rows", 1 << 61, "row count"), ("cols", 0, "columns"), ("cols", -5, "columns"), ("p", 1.0, "probability"),
                           ("p", -0.1, "probability"), ("p", float("nan"), "probability"), ("row0", -1, "row0"), ("row0", 1 << 60, "row0"),
                           ("step", (1 << 20) + 4, "step"), ("x", None, "x is null"), ("x", (1 << 20) + 2, "aligned"), ("ldx", 63, "apart"),
-                          ("ldx", -64, "apart"), ("ldx", 1 << 62, "stride"))]
+                          ("ldx", -64, "apart"), ("ldx", 1 << 62, "stride"), ("ldx", (1 << 40) + 1, "stride"))]
 BAD += [(f, "cols", 8193, "8192") for f in ("agcn_layer_norm", "agcn_layer_norm_backward")]
 BAD += [("agcn_layer_norm", k, v, word) for k, v, word in (("eps", 0.0, "eps"), ("eps", -1.0, "eps"), ("eps", float("nan"), "eps"), ("eps", 1e-40, "eps"),
                                                             ("eps", float("inf"), "eps"), ("y", None, "y is null"), ("ldy", 1, "apart"),

@@ -384,6 +384,35 @@ def test_calls_on_another_stream():
         del y2, got, late
 
 
+def test_calls_behind_an_event_of_another_stream():
+    # launched early behind what is before them on their own stream, but not ahead of the event that the stream waits for
+    from accelgcn import dropout, norm
+    require_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    _, x = _features(5_000, 64, F32, gen)
+    w, mask = torch.randn(64, generator=gen, device="cuda"), dict(p=0.5, seed=1)
+    y, d = norm.layer_norm(x, w, relu=True, **mask), dropout.dropout(x, **mask)
+    one, two, busy = torch.cuda.Stream(), torch.cuda.Stream(), torch.ones(1 << 26, device="cuda")
+    small = torch.zeros((16, 64), device="cuda")
+    late = torch.zeros_like(x)
+    for _ in range(5):
+        late.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            for _ in range(10):
+                busy.mul_(1.0)
+            late.copy_(x)
+            ready = torch.cuda.Event()
+            ready.record()
+        with torch.cuda.stream(two):
+            dropout.dropout(small, p=0.5, seed=1, out=small)        # a launch in front of the wait
+            two.wait_event(ready)
+            a = norm.layer_norm(late, w, relu=True, **mask)
+            b = dropout.dropout(late, **mask)
+        torch.cuda.synchronize()
+        assert torch.equal(a, y) and torch.equal(b, d)
+
+
 def test_elements_beyond_32_bits():
     from accelgcn import dropout, norm
     require_cuda()
@@ -517,7 +546,7 @@ def test_python_refusals():
                         (lambda: norm.layer_norm(x.t()), ValueError), (lambda: norm.layer_norm(x[:1].expand(6, 8)), ValueError),
                         (lambda: norm.layer_norm(x, w.half()), TypeError), (lambda: norm.layer_norm(x, w[:7]), ValueError),
                         (lambda: norm.layer_norm(x, w.cpu()), TypeError), (lambda: norm.layer_norm(x, out=x[:5]), ValueError),
-                        (lambda: norm.layer_norm(x, out=x.half()), ValueError), (lambda: norm.layer_norm(x, stats=s.t()), ValueError),
+                        (lambda: norm.layer_norm(x, out=x.half()), ValueError), (lambda: norm.layer_norm(x, stats=s.t()), ValueError), (lambda: norm.layer_norm(x, stats=s.view(2, 6)), ValueError),
                         (lambda: norm.layer_norm(x, stats=s.half()), TypeError), (lambda: norm.layer_norm(x, p=1.0), AccelGcnError),
                         (lambda: norm.layer_norm(x, eps=0), AccelGcnError), (lambda: norm.layer_norm(x, p=0.5, seed=1.0), TypeError),
                         (lambda: norm.layer_norm(x, step=torch.zeros(1, device="cuda")), TypeError),
