@@ -24,7 +24,7 @@ __device__ __noinline__ uint32_t closed_in_64_bits(const T *row, const float *we
 }
 
 template <typename T, int L, int CH, int LAYOUT>
-__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS, L > 0 && CH * Elem<T>::E <= 8 ? 2 : 1)
+__global__ void __launch_bounds__(L > 0 ? NORM_THREADS : NORM_MAX_THREADS, L > 0 && CH * Elem<T>::E <= (LAYOUT == ROWS_WHOLE ? 12 : 8) ? 2 : 1)
 layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
 {
     constexpr int E = Elem<T>::E;

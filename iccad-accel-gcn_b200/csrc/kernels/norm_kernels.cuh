@@ -173,7 +173,7 @@ __device__ __forceinline__ float inverse_sqrt(float v)
 template <int CH, int E>
 __device__ __forceinline__ void drop(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, float (&v)[CH][E])
 {
-    constexpr int AT_ONCE = CH > 1 ? CH / 2 : 1;             // half of them at once: all take the registers of a third of the warps
+    constexpr int AT_ONCE = CH * E == 16 ? CH / 2 : CH;      // 16 elements in two halves: all at once take the registers of other rows
 #pragma unroll
     for (int i = 0; i < CH; i += AT_ONCE) {
         int64_t blocks[AT_ONCE];

@@ -5,6 +5,7 @@
 namespace agcn {
 
 struct NormForwardLaunch {
+    static constexpr int ELEMS = NORM_FORWARD_ELEMS;
     NormForward &p;
     const NormForm &f;
     cudaStream_t s;

@@ -3,13 +3,16 @@
 #include "rows.h"
 #include "kernels/norm_kernels.cuh"
 
+#include <type_traits>
+
 namespace agcn {
 
 constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
-// Elements of a row per lane that a group within a warp aims at: 16 forward (with 8, 47 instructions per element in place of 29: 600 us for
-// 2 400 000 x 128 in place of 435); 8 backward, where 16 take over 200 registers.
-constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 8;
+// Elements of a row per lane that a group within a warp has at most: 16 forward (with 8, 47 instructions per element in place of 29: 600 us
+// for 2 400 000 x 128 in place of 435); 12 backward in 32 bits and 8 in 16, where 16 take over 200 registers (2 000 000 x 96: 496 us with 8,
+// 424-442 with 12).  Three chunks per lane where that is enough: 2 000 000 x 96 forward 324 -> 279 us, 200 000 x 700 309 -> 252.
+constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 12;
 // Backward pass: a call whose groups would have up to so many rows in turn runs as one cluster, which adds up the columns itself: 8 where a
 // row is a group's within a warp (2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace), 2 where it takes a thread
 // block (64 rows of 8 192: 29 us as 8 turns of 8, 19 as 64 thread blocks and a second kernel).
@@ -37,15 +40,13 @@ inline NormForm norm_form_of(int layout, int64_t cols, int dtype, int per_lane, 
     if (f.layout == ROWS_LOOSE) shift = 0;
     const int chunks = (int)ceil_div(cols + shift, e);
     f.lanes = 2;
-    while (f.lanes < 32 && f.lanes * per_lane / e < chunks) f.lanes *= 2;
+    while (f.lanes < 32 && f.lanes * (per_lane / e) < chunks) f.lanes *= 2;
     f.threads = NORM_THREADS;
     f.chunks = (int)ceil_div(chunks, f.lanes);
     if (f.chunks > most_chunks) {
         f.lanes = 0;
-        f.chunks = most_chunks;
         f.threads = 32 * (int)ceil_div(chunks, 32 * most_chunks);
-    } else if (f.chunks == 3) {
-        f.chunks = 4;
+        f.chunks = (int)ceil_div(chunks, f.threads) < 3 ? most_chunks : (int)ceil_div(chunks, f.threads);
     }
     f.rows_per_block = f.lanes > 0 ? NORM_THREADS / f.lanes : 1;
     return f;
@@ -66,15 +67,22 @@ inline int64_t norm_grid(const NormForm &f, int64_t rows, int64_t resident)
     return needed < resident ? needed : resident;
 }
 
-// Calls launch.template operator()<T, L, CH, LAYOUT>() of the form.
-template <typename T, int LAYOUT, int L, typename F> int norm_dispatch_chunks(const NormForm &f, F &&launch)
+// Whether norm_form_of() gives groups of L lanes with CH chunks each, `aim` of them aimed at and `most` the most.
+constexpr bool norm_reaches(int L, int CH, int aim, int most)
 {
-    constexpr int MOST = NORM_ELEMS / Elem<T>::E;
-    if constexpr (L > 0) {
-        if (f.chunks == 1) return launch.template operator()<T, L, 1, LAYOUT>();
-        if constexpr (MOST == 4) if (f.chunks == 2) return launch.template operator()<T, L, 2, LAYOUT>();
-    }
-    return launch.template operator()<T, L, MOST, LAYOUT>();
+    if (L == 0) return CH == most || CH == 3;
+    const int least = L == 2 ? 1 : L / 2 * aim + 1, top = L == 32 ? L * most : L * aim;      // chunks of a row
+    return CH >= (least + L - 1) / L && CH <= (top + L - 1) / L;
+}
+
+// Calls launch.template operator()<T, L, CH, LAYOUT>() of the form.
+template <typename T, int LAYOUT, int L, int CH = 1, typename F> int norm_dispatch_chunks(const NormForm &f, F &&launch)
+{
+    constexpr int MOST = NORM_ELEMS / Elem<T>::E, AIM = std::decay_t<F>::ELEMS / Elem<T>::E;
+    if constexpr (norm_reaches(L, CH, AIM, MOST)) if (f.chunks == CH) return launch.template operator()<T, L, CH, LAYOUT>();
+    if constexpr (CH < MOST) return norm_dispatch_chunks<T, LAYOUT, L, CH + 1>(f, launch);
+    set_error("no form of %d lanes and %d chunks", f.lanes, f.chunks);
+    return AGCN_ERR_INVALID;
 }
 template <typename T, int LAYOUT, typename F> int norm_dispatch_lanes(const NormForm &f, F &&launch)
 {

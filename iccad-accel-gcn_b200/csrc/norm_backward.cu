@@ -24,6 +24,7 @@ static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int sms)
 }
 
 struct NormBackwardLaunch {
+    static constexpr int ELEMS = NORM_BACKWARD_ELEMS;
     NormBackward &p;
     const NormForm &f;
     float *work;

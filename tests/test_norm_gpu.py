@@ -119,6 +119,26 @@ def test_few_rows_whose_columns_one_cluster_adds_up(rows, cols, t):
     _case(rows, cols, t, relu=True, p=0.25, weight=True, bias=True)
 
 
+@pytest.mark.parametrize("t", [F32, B16])
+def test_every_form_of_every_width(t):
+    # each number of lanes and chunks that a width can take, rows on and off 16-byte boundaries
+    from accelgcn import norm
+    require_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    for cols in [*range(1, 260), *range(260, 1100, 7), *range(1100, 8193, 131), 8185, 8186, 8191, 8192]:
+        x = torch.randn((9, cols + 3), generator=gen, device="cuda").to(t)[:, cols % 3:][:, :cols]
+        w, b = torch.randn(cols, generator=gen, device="cuda"), torch.randn(cols, generator=gen, device="cuda")
+        keep = torch.ones_like(x, dtype=torch.bool)
+        want, _, _, bound = rowwise.forward(x, w, b, 1e-5, True, 0.0, keep)
+        stats = torch.empty((9, 2), device="cuda")
+        out = torch.empty((9, cols + 3), dtype=t, device="cuda")[:, cols % 3:][:, :cols]
+        rowwise.check(f"y {cols}", norm.layer_norm(x, w, b, relu=True, stats=stats, out=out), want, bound)
+        dx, dw, db = norm.layer_norm_backward(x, x, stats, w, b, relu=True, dx=out)
+        ref = rowwise.backward(x, x, stats, w, b, True, 0.0, keep)
+        for name, got in (("dx", dx), ("dweight", dw), ("dbias", db)):
+            rowwise.check(f"{name} {cols}", got, *ref[name])
+
+
 def test_drawn_cases():
     rng = random.Random(20260)
     for _ in range(40):
@@ -283,34 +303,37 @@ def test_same_bits_from_run_to_run():
                 assert torch.equal(a, c)
 
 
-def test_column_sums_alone_and_left_out():
+@pytest.mark.parametrize("rows", [3000, 9000])           # one cluster, without a workspace; thread blocks of their own, with one
+def test_column_sums_alone_and_left_out(rows):
     from accelgcn import _lib, norm
     require_cuda()
     gen = torch.Generator(device="cuda").manual_seed(13)
-    _, x = _features(3000, 48, F32, gen)
-    _, dy = _features(3000, 48, F32, gen)
+    _, x = _features(rows, 48, F32, gen)
+    _, dy = _features(rows, 48, F32, gen)
     w, b, stats = torch.randn(48, generator=gen, device="cuda"), torch.randn(48, generator=gen, device="cuda"), _stats(x, 1e-5)
     dx, dw, db = norm.layer_norm_backward(dy, x, stats, w, b)
     # without a weight, the gradient that it would have had; none wanted
     got = norm.layer_norm_backward(dy, x, stats, None, b, dweight=torch.empty(48, device="cuda"))
     assert torch.equal(got[1], dw) and torch.equal(got[2], db)
     lib, dev = _lib.load(), torch.cuda.current_stream().cuda_stream
+    n = ctypes.c_int64()
+    _lib.check(lib.agcn_layer_norm_backward_work(rows, 48, 0, ctypes.byref(n)))
+    assert (n.value > 0) == (rows == 9000)
     out = torch.empty_like(dx)
     for pw, pb in ((None, None), (torch.empty(48, device="cuda"), None), (None, torch.empty(48, device="cuda"))):
-        n = ctypes.c_int64()
-        _lib.check(lib.agcn_layer_norm_backward_work(3000, 48, 0, ctypes.byref(n)))
         work = torch.full((n.value // 4 + 1,), float("nan"), device="cuda")
         none = pw is None and pb is None
         _lib.check(lib.agcn_layer_norm_backward(dy.data_ptr(), 48, x.data_ptr(), 48, stats.data_ptr(), w.data_ptr(), b.data_ptr(), out.data_ptr(), 48,
                                                 pw.data_ptr() if pw is not None else None, pb.data_ptr() if pb is not None else None,
-                                                None if none else work.data_ptr(), 0 if none else n.value, 3000, 48, 0, 0, 0.0, 0, 0, None, 0, dev))
+                                                None if none else work.data_ptr(), 0 if none else n.value, rows, 48, 0, 0, 0.0, 0, 0, None, 0, dev))
         assert torch.equal(out, dx) and (pw is None or torch.equal(pw, dw)) and (pb is None or torch.equal(pb, db))
         assert bool(torch.isnan(work[-1]))
-    # a workspace that is too small is refused, and nothing is written
-    out.fill_(float("nan"))
-    rc = lib.agcn_layer_norm_backward(dy.data_ptr(), 48, x.data_ptr(), 48, stats.data_ptr(), w.data_ptr(), b.data_ptr(), out.data_ptr(), 48, dw.data_ptr(),
-                                      db.data_ptr(), work.data_ptr(), n.value - 4, 3000, 48, 0, 0, 0.0, 0, 0, None, 0, dev)
-    assert rc == _lib.ERR_INVALID and b"workspace" in lib.agcn_last_error() and bool(torch.isnan(out).all())
+    if n.value:
+        # a workspace that is too small is refused, and nothing is written
+        out.fill_(float("nan"))
+        rc = lib.agcn_layer_norm_backward(dy.data_ptr(), 48, x.data_ptr(), 48, stats.data_ptr(), w.data_ptr(), b.data_ptr(), out.data_ptr(), 48, dw.data_ptr(),
+                                          db.data_ptr(), work.data_ptr(), n.value - 4, rows, 48, 0, 0, 0.0, 0, 0, None, 0, dev)
+        assert rc == _lib.ERR_INVALID and b"workspace" in lib.agcn_last_error() and bool(torch.isnan(out).all())
 
 
 def test_captured_steps_have_masks_of_their_own():
