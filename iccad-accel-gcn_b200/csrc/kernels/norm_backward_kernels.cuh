@@ -162,7 +162,7 @@ layer_norm_backward_kernel(const __grid_constant__ NormBackward p)
         x += p.x_step;
         dy += p.dy_step;
         if (p.mask.on) {
-            drop<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, g);
+            drop<L, CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, g);
         }
         if (live) {
 #pragma unroll

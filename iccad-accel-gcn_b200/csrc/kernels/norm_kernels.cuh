@@ -170,9 +170,19 @@ __device__ __forceinline__ float inverse_sqrt(float v)
 }
 
 // Zeroes what the mask drops of a thread's chunks; the first begins in block `block`, the next `stride` blocks later.
-template <int CH, int E>
+template <int L, int CH, int E>
 __device__ __forceinline__ void drop(const DropoutMask &m, int64_t offset, int64_t block, int stride, int skip, float (&v)[CH][E])
 {
+    // one answer for the warp: its groups may differ
+    if (__any_sync(0xffffffffu, skip != 0)) {
+        uint32_t bits[CH];
+        draw_bits<L, CH, E>(m, offset, block, stride, skip, (int)threadIdx.x & (L > 0 ? L - 1 : 31), bits);
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[j][e] = bits[j] >> e & 1u ? v[j][e] : 0.f;
+        return;
+    }
     constexpr int AT_ONCE = CH * E == 16 ? CH / 2 : CH;      // 16 elements in two halves: all at once take the registers of other rows
 #pragma unroll
     for (int i = 0; i < CH; i += AT_ONCE) {
@@ -180,7 +190,7 @@ __device__ __forceinline__ void drop(const DropoutMask &m, int64_t offset, int64
         uint32_t word[AT_ONCE][E];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; j++) blocks[j] = block + (i + j) * stride;
-        draw_words<AT_ONCE, E>(m, offset, blocks, skip, word);
+        draw_words<AT_ONCE, E>(m, offset, blocks, 0, word);
 #pragma unroll
         for (int j = 0; j < AT_ONCE; j++)
 #pragma unroll
@@ -308,7 +318,7 @@ layer_norm_kernel(const __grid_constant__ NormForward p)
                 for (int e = 0; e < E; e++) d[j][e] = relu_of(d[j][e]);
         }
         if (p.mask.on) {
-            drop<CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, d);
+            drop<L, CH, E>(p.mask, offset, block, at.lanes * (E / 4), skip, d);
         }
         if (live) {
             if (p.stats != nullptr && at.t == 0) *stats = make_float2(m + off, s);
