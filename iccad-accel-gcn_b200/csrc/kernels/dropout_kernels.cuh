@@ -28,21 +28,29 @@ struct DropoutParams {
 };
 
 // What becomes of U chunks that are in registers: elements lo .. hi - 1 of each (WHOLE: all E of them) are stored, at to[u] on.  Their
-// words begin with word `skip` of block[u].
-template <typename T, bool VEC, bool GATE, bool WHOLE, int U>
+// words begin with word `skip` of block[u].  WARP: all lanes of the warp call, with consecutive chunks and the same skip.
+template <typename T, bool VEC, bool GATE, bool WHOLE, bool WARP, int U>
 __device__ __forceinline__ void dropout_finish(const DropoutParams &p, int64_t offset, T *const (&to)[U], const int64_t (&block)[U], int skip, int lo, int hi,
                                                const uint4 (&v)[U], const uint4 (&gate)[GATE ? U : 1])
 {
     constexpr int E = Elem<T>::E;
     constexpr int AT_ONCE = E == 8 && U > 2 ? U / 2 : U;         // chunks whose words are made side by side
+    uint32_t bits[U];
+    const bool by_bits = WARP && p.mask.on && skip != 0;
+    if (by_bits) draw_bits<0, U, E>(p.mask, offset, block[0], block[U - 1 > 0 ? 1 : 0] - block[0], skip, (int)threadIdx.x & 31, bits);
 #pragma unroll
     for (int i = 0; i < U; i += AT_ONCE) {
         uint32_t word[AT_ONCE][E];
-        if (p.mask.on) {
+        if (by_bits) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+                for (int e = 0; e < E; e++) word[u][e] = bits[i + u] >> e & 1u ? ~0u : 0u;
+        } else if (p.mask.on) {
             int64_t these[AT_ONCE];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) these[u] = block[i + u];
-            draw_words<AT_ONCE, E>(p.mask, offset, these, skip, word);
+            draw_words<AT_ONCE, E>(p.mask, offset, these, WARP ? 0 : skip, word);
         }
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++) {
@@ -85,7 +93,7 @@ __device__ __forceinline__ void dropout_alone(const DropoutParams &p, int64_t of
     }
     T *to[1] = {out + at};
     const int64_t block[1] = {(p.mask.first + at) >> 2};
-    dropout_finish<T, true, GATE, false, 1>(p, offset, to, block, skip, lo, hi, v, gate);
+    dropout_finish<T, true, GATE, false, false, 1>(p, offset, to, block, skip, lo, hi, v, gate);
 }
 
 // Tensors that are one array of n elements each, and sit alike: chunks one behind the other, whatever the width.
@@ -102,8 +110,9 @@ dropout_array_kernel(const __grid_constant__ DropoutParams p)
     const int64_t step = (int64_t)gridDim.x * DROPOUT_THREADS * E;
     int64_t at = ((int64_t)blockIdx.x * DROPOUT_THREADS + threadIdx.x) * E - shift;
     const int skip = (int)((p.mask.first + at) & 3);
-    if (at < 0) {                              // the first few elements, in front of a boundary
-        dropout_alone<T, GATE>(p, offset, v_base, gate_base, out, at, n, skip);
+    // A warp stays together, so that its chunks are consecutive: where its first one begins in front of the array, ...
+    if (__any_sync(0xffffffffu, at < 0)) {
+        if (at < n) dropout_alone<T, GATE>(p, offset, v_base, gate_base, out, at, n, skip);
         at += step;
     }
     // U chunks at a time; the next ones are under way while these are worked on
@@ -115,7 +124,8 @@ dropout_array_kernel(const __grid_constant__ DropoutParams p)
             if (GATE) gate[GATE ? u : 0] = *reinterpret_cast<const uint4 *>(gate_base + a + u * step);
         }
     };
-    const int64_t span = (U - 1) * step + E;
+    // ... and where its last one is not all there any more
+    const int64_t span = (U - 1) * step + E + (31 - ((int)threadIdx.x & 31)) * E;
     if (at + span <= n) load(at);
     for (; at + span <= n; at += U * step) {
         uint4 these[U], its_gate[GATE ? U : 1];
@@ -129,7 +139,7 @@ dropout_array_kernel(const __grid_constant__ DropoutParams p)
             block[u] = ((p.mask.first + at) >> 2) + u * (step / 4);
         }
         if (at + U * step + span <= n) load(at + U * step);
-        dropout_finish<T, true, GATE, true, U>(p, offset, to, block, skip, 0, E, these, its_gate);
+        dropout_finish<T, true, GATE, true, true, U>(p, offset, to, block, skip, 0, E, these, its_gate);
     }
     for (; at < n; at += step) dropout_alone<T, GATE>(p, offset, v_base, gate_base, out, at, n, skip);
 }
@@ -212,7 +222,7 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
                 if (GATE) gate_from += gate_step;
             }
             if (k + U <= turns) {
-                dropout_finish<T, VEC, GATE, WHOLE, U>(p, offset, to, block, (int)(number & 3), lo, hi, v, gate);
+                dropout_finish<T, VEC, GATE, WHOLE, false, U>(p, offset, to, block, (int)(number & 3), lo, hi, v, gate);
             } else {
                 // the last rows, fewer than U
 #pragma unroll
@@ -221,7 +231,7 @@ dropout_rows_kernel(const __grid_constant__ DropoutParams p)
                     T *last[1] = {to[u]};
                     const int64_t its[1] = {block[u]};
                     const uint4 x[1] = {v[u]}, g[1] = {gate[GATE ? u : 0]};
-                    dropout_finish<T, VEC, GATE, WHOLE, 1>(p, offset, last, its, (int)(number & 3), lo, hi, x, g);
+                    dropout_finish<T, VEC, GATE, WHOLE, false, 1>(p, offset, last, its, (int)(number & 3), lo, hi, x, g);
                 }
             }
 #pragma unroll

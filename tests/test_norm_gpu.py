@@ -139,6 +139,33 @@ def test_every_form_of_every_width(t):
             rowwise.check(f"{name} {cols}", got, *ref[name])
 
 
+@pytest.mark.parametrize("t,shift,row0", [(F32, 0, 1), (F32, 1, 0), (F32, 3, 2), (B16, 0, 3), (B16, 5, 1), (F16, 1, (1 << 35) + 1)])
+def test_large_arrays_that_begin_inside_a_block(t, shift, row0):
+    # long enough for several rounds of every warp: its chunks begin inside the generator's blocks, and in front of the array
+    from accelgcn import dropout, norm
+    require_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    rows, cols, mask = 90_001, 61, dict(p=0.35, seed=21, offset=4, row0=row0)
+
+    def make(fill=True):
+        whole = torch.full((rows * cols + 16,), float("nan"), dtype=t, device="cuda")
+        x = whole[shift:shift + rows * cols].view(rows, cols)
+        if fill:
+            x.copy_(torch.randn((rows, cols), generator=gen, device="cuda"))
+        return whole, x
+
+    (_, x), (_, dy), (whole, out) = make(), make(), make(False)
+    keep = torch.from_numpy(rowwise.kept(rows, cols, 0.35, 21, 4, row0)).cuda()
+    scale = 1.0 / (1.0 - 0.35)
+    for got, v in ((lambda: dropout.dropout(x, relu=True, out=out, **mask), torch.where(keep, x.double().clamp(min=0) * scale, 0.0)),
+                   (lambda: dropout.dropout_backward(dy, relu=True, x=x, out=out, **mask), torch.where(keep & (x > 0), dy.double() * scale, 0.0))):
+        off = 2 * rowwise.U * v.abs()
+        rowwise.check("dropout", got(), v, off + rowwise.rounding(v, off, t))
+        assert bool(torch.isnan(whole[:shift]).all()) and bool(torch.isnan(whole[shift + rows * cols:]).all())
+    want, _, _, bound = rowwise.forward(x, None, None, 1e-5, True, 0.35, keep)
+    rowwise.check("y", norm.layer_norm(x, relu=True, out=out, **mask), want, bound)
+
+
 def test_drawn_cases():
     rng = random.Random(20260)
     for _ in range(40):
