@@ -12,8 +12,8 @@
 // same columns in all of them: weights and the sums over the rows stay in registers, and rows of any width are read 16 bytes at a time
 // (500 000 rows of 61: 58 us forward, 75-80 backward; rows of tensors that do not sit alike are read element by element).
 // The next rows are under way in a ring in shared memory meanwhile (RowRing): with loads into registers the forward pass took 750 us and
-// the backward 2 057.  What bounds it next is the instructions that can be issued: a layer's mask costs 15 per element, the rest 13
-// forward and 23-27 backward; in 16 bits, where a row is half the bytes, that is the bound (2 400 000 x 128 bf16: 360 and 540 us, 0.53 of the copy).
+// the backward 2 057.  What bounds it next is the instructions that can be issued: a layer's mask costs 14 to 16 per element, the
+// rest 11 forward and 25 backward; in 16 bits, where a row is half the bytes, that is the bound (2 400 000 x 128 bf16: 358 and 531 us, 0.53 of the copy).
 #pragma once
 #include "philox.cuh"
 #include "ptx.cuh"
