@@ -4,18 +4,19 @@
 
 namespace agcn {
 
-// Whether a call's thread blocks are one cluster
-static bool norm_one_cluster(int64_t rows, int64_t cols, int dtype)
+// Whether a call's thread blocks are one cluster.  `whole`: the form of rows that fill their chunks; `lanes`: those of the call's own form, which
+// is a thread block (0) for the widest rows that a warp has, where they begin behind a boundary (512 x 510 in fp32 as 64 turns of a cluster: 68 us,
+// 7.7 as thread blocks and a second kernel).
+static bool norm_one_cluster(int64_t rows, const NormForm &whole, int lanes)
 {
-    const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
-    return rows <= NORM_CLUSTER * (f.lanes > 0 ? NORM_CLUSTER_TURNS : NORM_CLUSTER_WIDE_TURNS) * f.rows_per_block;
+    return rows <= NORM_CLUSTER * (lanes > 0 ? NORM_CLUSTER_TURNS * whole.rows_per_block : NORM_CLUSTER_WIDE_TURNS);
 }
 
 // Thread blocks whose sums the workspace holds: all that are resident, for the forms there are
-static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int sms)
+static int64_t norm_parts(int64_t rows, int64_t cols, int dtype, int lanes, int sms)
 {
-    if (norm_one_cluster(rows, cols, dtype)) return 0;
     const NormForm f = norm_form_of(ROWS_WHOLE, cols, dtype, NORM_BACKWARD_ELEMS);
+    if (norm_one_cluster(rows, f, lanes)) return 0;
     // What a thread block writes for its columns (8 bytes each) should be little beside the rows that it reads: 16 of them at
     // least, but two thread blocks per SM where there are few rows.
     const int64_t resident = sms * (2048 / f.threads), few = 2 * sms > rows / 16 ? 2 * sms : rows / 16;
@@ -82,8 +83,11 @@ extern "C" int agcn_layer_norm_backward_work(int64_t rows, int64_t cols, int dty
     int dev = 0, sms = 0;
     int rc = check_sizes(who, rows, cols, NORM_MAX_COLS, dtype, AGCN_ACT_NONE);
     if (rc == AGCN_OK) rc = current_sm_count(&dev, &sms);
-    if (rc == AGCN_OK) *bytes = norm_parts(rows, cols, dtype, sms) * 2 * cols * (int64_t)sizeof(float);
-    return rc;
+    if (rc != AGCN_OK) return rc;
+    // wherever the rows begin: as far behind a boundary as they can
+    const NormForm f = norm_form_of(ROWS_EDGES, cols, dtype, NORM_BACKWARD_ELEMS, 16 / dtype_bytes(dtype) - 1);
+    *bytes = norm_parts(rows, cols, dtype, f.lanes, sms) * 2 * cols * (int64_t)sizeof(float);
+    return AGCN_OK;
 }
 
 extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const float *d_stats, const float *d_weight,
@@ -113,7 +117,8 @@ extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const vo
         if ((rc = check_rows(who, r, rows, cols, dtype)) != AGCN_OK) return rc;
     int dev = 0, sms = 0;
     if ((rc = current_sm_count(&dev, &sms)) != AGCN_OK) return rc;
-    const int64_t parts = norm_parts(rows, cols, dtype, sms);
+    const NormForm f = norm_form(t, 3, cols, dtype, NORM_BACKWARD_ELEMS);
+    const int64_t parts = norm_parts(rows, cols, dtype, f.lanes, sms);
     AGCN_REQUIRE((d_dweight == nullptr && d_dbias == nullptr) || parts == 0 || (d_work != nullptr && work_bytes >= parts * 2 * cols * (int64_t)sizeof(float)),
                  "%s: workspace of %lld bytes, %lld are needed", who, (long long)work_bytes, (long long)(parts * 2 * cols * (int64_t)sizeof(float)));
     a.dy = d_dy; a.lddy = lddy; a.x = d_x; a.ldx = ldx; a.dx = d_dx; a.lddx = lddx; a.rows = rows;
@@ -122,6 +127,5 @@ extern "C" int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const vo
     a.dweight = d_dweight; a.dbias = d_dbias;
     a.cols = (int)cols; a.relu = activation == AGCN_ACT_RELU;
     a.inv_cols = 1.f / (float)cols;
-    const NormForm f = norm_form(t, 3, cols, dtype, NORM_BACKWARD_ELEMS);
     return norm_dispatch(f, dtype, NormBackwardLaunch{a, f, static_cast<float *>(d_work), parts, s});
 }

@@ -1,0 +1,52 @@
+"""Column sums of the layer norm's backward pass: which calls need a workspace, sums that must be exact, rows off 16-byte boundaries
+over many turns."""
+import ctypes
+
+import pytest
+import torch
+
+from conftest import require_cuda
+from test_norm_gpu import _case
+
+pytestmark = pytest.mark.gpu
+
+F32, B16, F16 = torch.float32, torch.bfloat16, torch.float16
+CODES = {F32: 0, B16: 1, F16: 2}
+
+
+def _work(rows, cols, t):
+    from accelgcn import _lib
+    n = ctypes.c_int64()
+    _lib.check(_lib.load().agcn_layer_norm_backward_work(rows, cols, CODES[t], ctypes.byref(n)))
+    return n.value
+
+
+@pytest.mark.parametrize("rows,cols,t", [(512, 510, F32), (17, 511, F32), (512, 507, B16), (100, 511, F16)])
+def test_few_rows_of_a_thread_block_each_are_not_one_cluster(rows, cols, t):
+    # the widest rows that a warp has, where they begin behind a 16-byte boundary: a thread block has one, and a cluster would have up to
+    # 64 of them in turn.  (Once one, on 8 of the SMs, without a workspace.)
+    require_cuda()
+    assert _work(rows, cols, t) > 0 and _work(16, cols, t) == 0
+    _case(rows, cols, t, relu=True, p=0.25, weight=True, bias=True)
+    _case(16, cols, t, relu=True, p=0.25, weight=True, bias=True)
+
+
+@pytest.mark.parametrize("start,needed", [(0, False), (1, True)])
+def test_the_workspace_is_needed_where_the_rows_sit(start, needed):
+    # 512 columns on a boundary are a warp's: a cluster adds up 512 rows of them, as ever, and needs no workspace
+    from accelgcn import _lib
+    require_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    rows, cols = 300, 512
+    x, dy, dx = (torch.randn((rows, cols + 4), generator=gen, device="cuda")[:, start:start + cols] for _ in range(3))
+    stats = torch.ones((rows, 2), device="cuda")
+    dw, db = torch.full((cols,), 7.0, device="cuda"), torch.empty(cols, device="cuda")
+    rc = _lib.load().agcn_layer_norm_backward(dy.data_ptr(), cols + 4, x.data_ptr(), cols + 4, stats.data_ptr(), None, None, dx.data_ptr(), cols + 4,
+                                              dw.data_ptr(), db.data_ptr(), None, 0, rows, cols, 0, 0, 0.0, 0, 0, None, 0,
+                                              torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    if needed:
+        assert rc == _lib.ERR_INVALID and b"workspace" in _lib.load().agcn_last_error() and bool((dw == 7.0).all())
+    else:
+        assert rc == _lib.OK
+        assert bool(((db - dy.double().sum(0)).abs() <= 300 * 2.0 ** -24 * dy.double().abs().sum(0)).all())
