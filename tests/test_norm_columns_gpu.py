@@ -50,3 +50,21 @@ def test_the_workspace_is_needed_where_the_rows_sit(start, needed):
     else:
         assert rc == _lib.OK
         assert bool(((db - dy.double().sum(0)).abs() <= 300 * 2.0 ** -24 * dy.double().abs().sum(0)).all())
+
+
+def test_a_term_of_few_rows_has_few_roundings_behind_it():
+    # 2 048 rows of 16: two rows per group of a thread block of 128, 8 thread blocks.  Behind a term are at most 1 addition in its thread, 15 + 3
+    # among the groups and 3 among the thread blocks.  One large term in each thread block, on which a 1 is a tie that is rounded away each
+    # time: 127 in turn would be off by 127 U.
+    from accelgcn import norm
+    require_cuda()
+    dy = torch.ones((2048, 16), device="cuda")
+    dy[1024:] = 0.0
+    dy[:1024:128] = 2.0 ** 24
+    x = torch.ones_like(dy)
+    stats = torch.tensor([[0.0, 1.0]], device="cuda").repeat(2048, 1)
+    w = torch.ones(16, device="cuda")
+    _dx, dw, db = norm.layer_norm_backward(dy, x, stats, w, w)
+    want = dy.double().sum(0)
+    for got in (dw, db):                          # h = 1: the two sums are the same
+        assert bool(((got - want).abs() <= 22 * 2.0 ** -24 * want).all()), float(((got - want).abs() / want).max() * 2.0 ** 24)
