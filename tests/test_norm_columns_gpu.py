@@ -68,3 +68,58 @@ def test_a_term_of_few_rows_has_few_roundings_behind_it():
     want = dy.double().sum(0)
     for got in (dw, db):                          # h = 1: the two sums are the same
         assert bool(((got - want).abs() <= 22 * 2.0 ** -24 * want).all()), float(((got - want).abs() / want).max() * 2.0 ** 24)
+
+
+def _signs(shape, t, gen):
+    return torch.randint(0, 2, shape, generator=gen, device="cuda", dtype=torch.int8).mul_(2).sub_(1).to(t)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("cols,t,rows_per_block", [(16, F32, 128), (61, F32, 32), (128, F32, 16), (100, B16, 16), (128, F16, 16), (500, F32, 8), (701, F32, 1),
+                                                   (1001, F32, 1), (1003, B16, 1)])
+def test_no_row_is_lost(cols, t, rows_per_block, p):
+    # terms of +1 and -1 (+2 and -2 with a mask): every sum on the way is a whole number below 2^24, so the result is exact, whatever
+    # the order.  The rows end before, with and behind a whole turn of all groups, for each number of thread blocks per SM.
+    import rowwise
+    from accelgcn import norm
+    require_cuda()
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    most = 5 * (4 * sms // 8 * 8) * rows_per_block + 1
+    xs, dys = _signs((most, cols), t, gen), _signs((most, cols), t, gen)
+    kept = torch.from_numpy(rowwise.kept(most, cols, p, 5, 0)).cuda()
+    stats = torch.tensor([[0.0, 1.0]], device="cuda").repeat(most, 1)
+    w, dx = torch.ones(cols, device="cuda"), torch.empty_like(xs)
+    for per_sm in (1, 2, 3, 4):
+        for more in (-1, 0, 1):
+            rows = 5 * (per_sm * sms // 8 * 8) * rows_per_block + more
+            x, dy = xs[:rows], dys[:rows]
+            _dx, dw, db = norm.layer_norm_backward(dy, x, stats[:rows], w, w, p=p, seed=5, dx=dx[:rows])
+            dz = torch.where(kept[:rows], dy.double(), 0.0) * (1.0 / (1.0 - p))
+            assert torch.equal(db.double(), dz.sum(0)) and torch.equal(dw.double(), (dz * x.double()).sum(0)), rows
+
+
+def test_no_row_is_lost_beyond_32_bits():
+    from accelgcn import norm
+    require_cuda()
+    rows, cols = 17_000_000, 128                 # 2.2e9 elements, 4.4 GB
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    gen = torch.Generator(device="cuda").manual_seed(33)
+    x, dy = _signs((rows, cols), B16, gen), _signs((rows, cols), B16, gen)
+    stats = torch.tensor([[0.0, 1.0]], device="cuda").repeat(rows, 1)
+    w = torch.ones(cols, device="cuda")
+    _dx, dw, db = norm.layer_norm_backward(dy, x, stats, w, w)
+    dw64, db64 = torch.zeros(cols, dtype=torch.float64, device="cuda"), torch.zeros(cols, dtype=torch.float64, device="cuda")
+    for r in range(0, rows, 1_000_000):
+        part = slice(r, min(rows, r + 1_000_000))
+        db64 += dy[part].double().sum(0)
+        dw64 += (dy[part].double() * x[part].double()).sum(0)
+    assert torch.equal(db.double(), db64) and torch.equal(dw.double(), dw64)
+
+
+@pytest.mark.parametrize("rows,cols,t,row0", [(20_000, 1001, F32, 1), (20_003, 1003, B16, 0), (20_000, 701, F32, 3), (20_001, 511, F32, 0), (12_000, 2046, F16, 1)])
+def test_many_rows_of_a_thread_block_each_off_the_boundary(rows, cols, t, row0):
+    # 17 and more rows in turn per thread block: the ring is filled anew by chunks that the row does not fill, and the mask's words
+    # go from lane to lane, row after row
+    _case(rows, cols, t, relu=True, p=0.5, weight=True, bias=True, row0=row0)
