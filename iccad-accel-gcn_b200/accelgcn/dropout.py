@@ -5,7 +5,7 @@ agcn_dropout / agcn_dropout_backward.
     dy = dropout.dropout_backward(dh, p=0.5, seed=seed, offset=step, relu=True, x=y)      # x: what went in, or relu of it
 
 The mask is made from (seed, offset, the element's number) in both passes and never stored: give every layer and step another
-offset, and both passes of one the same.
+offset, and both passes of one the same.  These are plain functions on tensors: autograd does not see them.
 """
 from __future__ import annotations
 

@@ -27,7 +27,7 @@ _forward = _backward = None
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, relu: bool = False, p: float = 0.0, seed: int = 0, offset: int = 0,
                row0: int = 0, step=None, out=None, stats=None, stream=None):
     """dropout(relu(layer_norm(x) * weight + bias)) of x [rows, cols] (float32, bfloat16 or float16 CUDA, any row stride, at
-    most 8192 columns); weight and bias float32 [cols] or None.  relu and dropout (p > 0) are optional.  `stats`, float32
+    most 8192 columns); weight and bias float32 [cols] or None.  relu and dropout (p > 0) are optional; eps is 1e-30 to 1e30.  `stats`, float32
     [rows, 2], receives mean and 1 / sqrt(variance + eps) of the rows: what the backward pass needs.  row0: where this
     rank's rows begin in the whole.  step: an int64 on the device that is added to `offset` when the kernel runs (a captured
     graph counts it up to have new masks).  out may be x.  Asynchronous on the current stream (or `stream`)."""

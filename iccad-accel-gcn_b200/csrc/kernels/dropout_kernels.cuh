@@ -1,8 +1,8 @@
 // Dropout of features, with the ReLU before it, and their gradient:
 //     y = keep relu(v) / (1 - p)            dx = keep [x > 0] dy / (1 - p)
 // v is x or dy, gate the x of the second.  One pass over the tensors, a thread with 4 chunks of 16 bytes at a time so that
-// enough is under way.  The mask (philox.cuh) costs some 13 instructions per element: bound by HBM in 32 bits, by both
-// in 16.
+// enough is under way.  The mask (philox.cuh) costs some 13 instructions per element: bound by HBM in 32 bits; in
+// 16 by the mask at 16 warps per SM (57 to 62 % of the issue slots in use, DRAM at 3.8 TB/s forward and 5.2 back).
 #pragma once
 #include "philox.cuh"
 #include "ptx.cuh"

@@ -10,10 +10,13 @@
 // thread block) has a row at a time in registers, CH chunks of 16 bytes per lane, so every element is read once; rows go round-robin over
 // the groups.  The number of groups is a multiple of 8, so a group's rows all sit at one offset from a 16-byte boundary and a lane has the
 // same columns in all of them: weights and the sums over the rows stay in registers, and rows of any width are read 16 bytes at a time
-// (500 000 rows of 61: 58 us forward, 75-80 backward; rows of tensors that do not sit alike are read element by element).
+// (500 000 rows of 61: 58 us forward, 74-84 backward).  Rows of tensors that do not sit alike are read element by element, with none ahead:
+// 1 000 000 x 128 into a slice that begins one column later 271 us in place of 168 forward, 366 of 243 back; bf16 445 of 155, 359 of 227.
 // The next rows are under way in a ring in shared memory meanwhile (RowRing): with loads into registers the forward pass took 750 us and
-// the backward 2 057.  What bounds it next is the instructions that can be issued: a layer's mask costs 14 to 16 per element, the
-// rest 11 forward and 25 backward; in 16 bits, where a row is half the bytes, that is the bound (2 400 000 x 128 bf16: 358 and 531 us, 0.53 of the copy).
+// the backward 2 057.  What bounds it next is how fast 16 warps per SM get through their instructions: a layer's mask costs 14 to 16 per element, the
+// rest 11 forward and 25 backward, and a warp waits for the results of its own ones and for the half-rate units that the mask's multiplies and
+// exclusive ors need; 54 to 64 % of the issue slots are in use.  In 16 bits, where a row is half the bytes, that is the bound, and nothing
+// waits for memory (2 400 000 x 128 bf16: 358-365 and 531 us, 0.53 of the copy).
 #pragma once
 #include "philox.cuh"
 #include "ptx.cuh"

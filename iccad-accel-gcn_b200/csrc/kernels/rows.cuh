@@ -76,8 +76,8 @@ template <> struct Elem<__half> {
     }
 };
 
-// Two fp32 operations in one instruction (both rounded as the single ones are): these kernels are bound by the instructions
-// that can be issued long before the arithmetic units are full.
+// Two fp32 operations in one instruction (both rounded as the single ones are): fewer instructions for the few warps that there are
+// (2 400 000 x 128, layer norm: 435 -> 417 us, backward 650 -> 625-645).
 __device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
     float2 r;

@@ -11,11 +11,15 @@ constexpr int64_t NORM_MAX_COLS = AGCN_NORM_MAX_COLS;
 constexpr int NORM_ELEMS = 16;              // of a row per thread, at most
 // Elements of a row per lane that a group within a warp has at most: 16 forward (with 8, 47 instructions per element in place of 29: 600 us
 // for 2 400 000 x 128 in place of 435); 12 backward in 32 bits and 8 in 16, where 16 take over 200 registers (2 000 000 x 96: 496 us with 8,
-// 424-442 with 12).  Three chunks per lane where that is enough: 2 000 000 x 96 forward 324 -> 279 us, 200 000 x 700 309 -> 252.
+// 424-442 with 12).  That is what is aimed at with fewer than 32 lanes; 32 go on to 16 elements (backward 385 to 512 columns in 32 bits, 257 to 512 in
+// 16) with 216 registers and one thread block per SM, since one warp as a thread block per row is slower with a mask: 200 000 x 512 fp32 194
+// us, 210 as that (185, 222 without a mask), 400 000 x 512 bf16 342, 364 (without a mask 241, 221), 400 000 x 384 bf16 347, 363.  Three chunks per lane where that is enough: 2 000 000 x 96 forward 324 -> 279 us, 200 000 x 700 309 -> 252.
 constexpr int NORM_FORWARD_ELEMS = 16, NORM_BACKWARD_ELEMS = 12;
 // Backward pass: a call whose groups would have up to so many rows in turn runs as one cluster, which adds up the columns itself: 8 where a
 // row is a group's within a warp (2 048 rows of 16: 7.9 us a call, 14.8 with a second kernel and a workspace), 2 where it takes a thread
-// block (64 rows of 8 192: 29 us as 8 turns of 8, 19 as 64 thread blocks and a second kernel).
+// block (64 rows of 8 192: 29 us as 8 turns of 8, 19 as 64 thread blocks and a second kernel).  Within a warp it goes by the groups that rows on a
+// 16-byte boundary have, because the workspace's size is asked for without the addresses: rows off it whose chunk more makes a group twice as wide
+// have up to 16 in turn (2 048 x 95: 18.0 us on the GPU; a workspace would make it 6.4).
 constexpr int NORM_CLUSTER_TURNS = 8, NORM_CLUSTER_WIDE_TURNS = 2;
 constexpr int NORM_MAX_SMEM = 200 * 1024;
 static_assert(NORM_MAX_THREADS * NORM_ELEMS * (norm_backward_stages(0) * 2 * 4 + 8) <= NORM_MAX_SMEM, "8192 columns in 32 bits");

@@ -471,7 +471,7 @@ int agcn_gcn2_forward_destroy(agcn_gcn2 *fwd);
 
 /* y = dropout(act((x - m) s * weight + bias)),  m and s = 1 / sqrt(variance + eps) those of each row of x (the variance
  * divides by cols).  weight / bias [cols] fp32, NULL: 1 / 0.  d_stats: NULL, or fp32 [rows x 2], contiguous, which
- * receives (m, s) for the backward pass.  1 <= cols <= AGCN_NORM_MAX_COLS.  Squares are taken in fp32: deviations from
+ * receives (m, s) for the backward pass.  1 <= cols <= AGCN_NORM_MAX_COLS, 1e-30 <= eps <= 1e30.  Squares are taken in fp32: deviations from
  * the mean of 1e19 and more overflow. */
 int agcn_layer_norm(const void *d_x, int64_t ldx, const float *d_weight, const float *d_bias, double eps,
                     void *d_y, int64_t ldy, float *d_stats, int64_t rows, int64_t cols, int dtype, int activation,
@@ -480,7 +480,7 @@ int agcn_layer_norm(const void *d_x, int64_t ldx, const float *d_weight, const f
 /* Its gradients, from dy, the x, stats, weight and bias of the forward pass, and the same activation and mask:
  * d_dx [rows x cols] of `dtype`, d_dweight and d_dbias [cols] fp32 (overwritten; either may be NULL).  The sums over
  * the rows are made in one order: the same bits from run to run on one GPU model.  d_work: fp32 workspace of at least
- * agcn_layer_norm_backward_work(...) bytes (what the current device needs; 0 for few rows), whose contents mean nothing before and
+ * agcn_layer_norm_backward_work(...) bytes (what the current device needs, wherever the rows begin; 0 for few rows), whose contents mean nothing before and
  * after; calls that may overlap need one each.  NULL where neither d_dweight nor d_dbias is wanted. */
 int agcn_layer_norm_backward_work(int64_t rows, int64_t cols, int dtype, int64_t *bytes);
 int agcn_layer_norm_backward(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const float *d_stats,
